@@ -7,6 +7,9 @@
  *   decode_splitk     the same with a fixed split count, emitting (m, l, o) softmax
  *                     partials per (sequence, q head, split)
  *   combine           merge partials into the attention output (or into one partial)
+ *   extend_attention  attention of SEVERAL new tokens per sequence over the packed cache
+ *   build_step        block tables, slots, positions and lengths of a step from request lengths
+ *   token_score       log probability, entropy, rank and top alternatives of given tokens
  *
  * Every entry point is plain C: raw device pointers, sizes, strides and a
  * cudaStream_t passed as void*.  Nothing here allocates or synchronises except
@@ -390,6 +393,97 @@ int knlp_b200_decode_noalloc(const void* query, int q_dtype, const int64_t q_str
                              int n_seqs, int n_q_heads, int n_kv_heads, int head_dim,
                              int block_size, int n_splits, int max_seq_len,
                              void* out, int out_dtype, int64_t out_row_stride, void* stream);
+
+/*
+ * Attention of several query tokens per sequence over the packed cache: chunked prefill,
+ * verification of drafted tokens, batches that mix both with single-token decodes.  (The
+ * reference serves these from an unquantized copy of the cache: forward :2746-2849, mixed
+ * batches split by query length.)  The new tokens are already in the cache.
+ *   query            [n_tokens, n_q_heads, head_dim] fp16 or bf16, the sequences' tokens one
+ *                    after another; q_stride = {token, head} in elements
+ *   query_start_loc  int32 [n_seqs + 1]: sequence s owns rows [loc[s], loc[s+1]); ascending,
+ *                    within [0, n_tokens].  Rows of no sequence are left as they were
+ *   seq_lens         int32 [n_seqs]: cached tokens INCLUDING the new ones.  Query token i of
+ *                    the n of a sequence stands at position len - n + i and attends to the
+ *                    positions up to its own; a row without any (len < n) gives 0
+ *   block_table      as knlp_b200_decode_splitk; max_blocks entries per row.  A length above
+ *                    max_blocks * block_size is cut there
+ *   max_query_len    host-known bounds of the new tokens per sequence and of seq_lens.  They
+ *   max_seq_len      choose how the work is split, never what is computed
+ *   softmax_scale    factor of the scores, > 0 (head_dim^-1/2 as a rule)
+ *   workspace        floats, >= what knlp_b200_extend_workspace reports; scratch.  Calls that
+ *                    may overlap on the GPU need one each
+ *   out              [n_tokens * n_q_heads, head_dim] of out_dtype, row stride out_row_stride
+ *   lse              NULL, or float [n_tokens * n_q_heads]: log of the sum of exp(scores), -inf
+ *                    for a row that attends to nothing
+ *   flags            KNLP_EXTEND_FULL: every query token attends to all cached tokens (a far
+ *                    segment that lies before the new tokens, merged by lse with the rest);
+ *                    KNLP_EXTEND_FORCE_GENERIC: the stride-generic CUDA-core kernel
+ * An unquantized K plane must have the query's type.
+ */
+#define KNLP_EXTEND_FORCE_GENERIC 1u
+#define KNLP_EXTEND_FULL 2u
+int knlp_b200_extend_workspace(int n_seqs, int n_tokens, int n_q_heads, int n_kv_heads,
+                               int head_dim, int64_t* workspace_floats_out);
+int knlp_b200_extend_attention(const void* query, int q_dtype, const int64_t q_stride[2],
+                               const knlp_kv_plane* k_plane, const knlp_kv_plane* v_plane,
+                               const int32_t* block_table, int64_t bt_stride, int max_blocks,
+                               const int32_t* seq_lens, const int32_t* query_start_loc,
+                               int64_t num_blocks, int n_seqs, int n_tokens, int n_q_heads,
+                               int n_kv_heads, int head_dim, int block_size, int max_query_len,
+                               int max_seq_len, float softmax_scale, float* workspace,
+                               int64_t workspace_floats, void* out, int out_dtype,
+                               int64_t out_row_stride, float* lse, unsigned flags, void* stream);
+
+/*
+ * Tables of a serving step, built on the GPU from the requests' lengths in one launch (what
+ * the reference takes ready-made from its scheduler, :2210-2252).
+ *   context_lens     int32 [n_seqs]: tokens of each request in the cache before the step
+ *   query_lens       int32 [n_seqs]: its new tokens (0 allowed); negative lengths count as 0
+ *   block_table      int32, rows of bt_stride; max_blocks entries per row.  The entries of a
+ *                    request's first ceil(context / block_size) blocks are read; those that
+ *                    its new tokens need beyond them are WRITTEN, all others stay
+ *   free_blocks      int32 [n_free]: ids of free cache blocks, taken from the front on in the
+ *                    order of the requests; free_head: NULL, or where the front is (int32 [1])
+ *   n_slots          rows of slot_mapping and positions, >= the step's new tokens; what lies
+ *                    behind the last token gets slot -1 and position 0
+ *   query_start_loc  int32 [n_seqs + 1] out; seq_lens: int32 [n_seqs] out, context + new
+ *   slot_mapping     int64 [n_slots] out: block * block_size + offset, the slot mapping of
+ *                    knlp_b200_quant_append; -1 for a token without a block
+ *   positions        NULL, or int64 [n_slots] out
+ *   blocks_taken     int32 [1] out: blocks the step needs.  If the free list holds fewer, the
+ *                    entries and slots behind its end are -1; needs beyond max_blocks of a
+ *                    row take no block
+ * Limits: n_slots and the new tokens of a step < 2^30, max_blocks <= 2^20.
+ */
+int knlp_b200_build_step(const int32_t* context_lens, const int32_t* query_lens,
+                         int32_t* block_table, int64_t bt_stride, int max_blocks,
+                         const int32_t* free_blocks, int64_t n_free, const int32_t* free_head,
+                         int n_seqs, int block_size, int64_t n_slots, int32_t* query_start_loc,
+                         int32_t* seq_lens, int64_t* slot_mapping, int64_t* positions,
+                         int32_t* blocks_taken, void* stream);
+
+/*
+ * Scores of given tokens from logits, one pass over them: what the evaluation harness and a
+ * server's log-probability output compute from a model's answer.
+ *   logits        [n_rows, vocab] of dtype, row stride row_stride elements (any alignment of
+ *                 whole elements); -inf masks a token
+ *   token_ids     int64 [n_rows]; a negative id gives logprob 0 and rank 0, one >= vocab NaN
+ *                 and rank 0
+ *   logprob       float [n_rows]: logit - log(sum(exp(logits)))
+ *   entropy       float [n_rows], in nats
+ *   rank          int32 [n_rows]: 1 + number of logits larger than the token's
+ *   top_ids       int64 [n_rows, top_k], top_logprobs float [n_rows, top_k]: the largest
+ *                 logits in descending order, the lower index first among equals (NULL when
+ *                 top_k is 0); top_k <= KNLP_MAX_TOP and <= vocab
+ * A row without a logit above -inf has entropy 0 and every log probability -inf; a NaN or +inf
+ * logit makes the row's logprob and entropy NaN, and NaN counts as the largest logit.
+ */
+#define KNLP_MAX_TOP 64
+int knlp_b200_token_score(const void* logits, int dtype, int64_t row_stride,
+                          const int64_t* token_ids, int n_rows, int vocab, int top_k,
+                          float* logprob, float* entropy, int32_t* rank, int64_t* top_ids,
+                          float* top_logprobs, void* stream);
 
 #ifdef __cplusplus
 }

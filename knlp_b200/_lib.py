@@ -24,6 +24,9 @@ DECODE_USE_TMA = 2
 DECODE_EMIT_PARTIAL = 4
 DECODE_FIXED_SPLITS = 8
 DECODE_DEBUG_STALL = 16
+EXTEND_FORCE_GENERIC = 1
+EXTEND_FULL = 2
+MAX_TOP = 64
 
 SYMBOLS = (
     "knlp_b200_abi_version",
@@ -42,6 +45,10 @@ SYMBOLS = (
     "knlp_b200_decode_noalloc",
     "knlp_b200_plugin_quantize",
     "knlp_b200_plugin_dequantize",
+    "knlp_b200_extend_workspace",
+    "knlp_b200_extend_attention",
+    "knlp_b200_build_step",
+    "knlp_b200_token_score",
 )
 
 
@@ -156,6 +163,24 @@ def load() -> C.CDLL:
     lib.knlp_b200_plugin_dequantize.restype = C.c_int
     lib.knlp_b200_plugin_dequantize.argtypes = [
         C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_void_p, C.c_void_p]
+    lib.knlp_b200_extend_workspace.restype = C.c_int
+    lib.knlp_b200_extend_workspace.argtypes = [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
+                                               C.POINTER(C.c_int64)]
+    lib.knlp_b200_extend_attention.restype = C.c_int
+    lib.knlp_b200_extend_attention.argtypes = [
+        C.c_void_p, C.c_int, I64P, PL, PL, C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_void_p,
+        C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
+        C.c_float, C.c_void_p, C.c_int64, C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_uint,
+        C.c_void_p]
+    lib.knlp_b200_build_step.restype = C.c_int
+    lib.knlp_b200_build_step.argtypes = [
+        C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_int64, C.c_void_p,
+        C.c_int, C.c_int, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+        C.c_void_p]
+    lib.knlp_b200_token_score.restype = C.c_int
+    lib.knlp_b200_token_score.argtypes = [
+        C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p,
+        C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
     if lib.knlp_b200_abi_version() != ABI_VERSION:
         raise RuntimeError("libknlp_b200.so ABI version mismatch; rebuild it")
     _lib = lib

@@ -15,19 +15,23 @@ pieces here:
     do_kv_cache_update            :2483-2546   cache write of a step's new tokens
     _fused_decode                 :2851-2928   decode dispatch over k_precision / v_precision
 
-The kernels behind it are this package's (``ops``); nothing here touches vLLM.  One
-addition the reference does not have: ``decode_step`` appends the step's token and
-attends in ONE launch when both planes are quantized (the reference writes, then decodes).
+The kernels behind it are this package's (``ops``); nothing here touches vLLM.  Additions
+that the reference does not have: ``decode_step`` appends the step's token and attends in ONE
+launch when both planes are quantized (the reference writes, then decodes); ``build_step``
+makes a step's block tables and slot maps on the GPU from the requests' lengths; ``extend`` /
+``forward`` attend with several new tokens per sequence over the packed cache (the reference's
+forward :2746-2849 does that over an unquantized copy).
 """
 
 from __future__ import annotations
 
+import ctypes as C
 from dataclasses import dataclass
 from typing import Optional, Tuple
 
 import torch
 
-from . import ops
+from . import _lib, ops
 
 GROUP_SIZE = ops.GROUP_SIZE
 
@@ -80,6 +84,65 @@ class AttentionMetadata:
     slot_mapping: torch.Tensor
 
 
+@dataclass
+class StepTables:
+    """What ``build_step`` makes of a step's request lengths."""
+    query_start_loc: torch.Tensor  # int32 [S + 1]
+    seq_lens: torch.Tensor  # int32 [S], with the new tokens
+    slot_mapping: torch.Tensor  # int64 [num_tokens], -1 = no token or no block
+    positions: torch.Tensor  # int64 [num_tokens]
+    blocks_taken: torch.Tensor  # int32 [1], blocks the step needs from the free list
+
+
+def build_step(context_lens: torch.Tensor, query_lens: torch.Tensor, block_table: torch.Tensor,
+               free_blocks: torch.Tensor, block_size: int, num_tokens: int, *,
+               free_head: Optional[torch.Tensor] = None) -> StepTables:
+    """Block tables and slot maps of a step, on the GPU in one launch.
+
+    context_lens, query_lens  int32 [S]: each request's tokens in the cache, and its new ones
+    block_table               int32 [S, max_blocks], updated IN PLACE: the entries of blocks that
+                              the new tokens need beyond ceil(context / block_size)
+    free_blocks               int32 [n]: ids of free blocks, taken in the order of the requests
+                              from ``free_head`` (int32 [1] on the GPU; default the front) on
+    num_tokens                rows of ``slot_mapping`` / ``positions``: the step's new tokens, or
+                              a padded count (rows behind the last token get slot -1)
+
+    Nothing is read back: the caller advances its free list by ``blocks_taken`` on the GPU, or
+    from the same arithmetic on the host.  Where the list or a table row is too short, the
+    tokens behind it get slot -1 and table entries -1, and ``blocks_taken`` exceeds the list."""
+    dev = ops._need_cuda(context_lens, query_lens, block_table, free_blocks, free_head)
+    S = context_lens.shape[0] if context_lens.dim() == 1 else -1
+    for t, shape, what in ((context_lens, (S,), "context_lens"), (query_lens, (S,), "query_lens"),
+                           (free_blocks, (free_blocks.numel(),), "free_blocks"),
+                           (free_head, (1,), "free_head")):
+        if t is None:
+            continue
+        if t.dtype != torch.int32:
+            raise TypeError(f"{what} must be int32")
+        if S < 0 or tuple(t.shape) != shape or not t.is_contiguous():
+            raise ValueError(f"{what} must be a contiguous vector of {shape[0]} elements")
+    if block_table.dtype != torch.int32:
+        raise TypeError("block_table must be int32")
+    if block_table.dim() != 2 or block_table.shape[0] != S or block_table.shape[1] == 0 or (
+            block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError("block_table must be [S, max_blocks] with contiguous rows")
+    if block_size <= 0 or num_tokens < 0:
+        raise ValueError("block_size must be positive and num_tokens not negative")
+    small = torch.empty(2 * S + 2, dtype=torch.int32, device=dev)
+    wide = torch.empty((2, num_tokens), dtype=torch.int64, device=dev)
+    starts, lens, taken = small[:S + 1], small[S + 1:2 * S + 1], small[2 * S + 1:]
+    slots, positions = wide[0], wide[1]
+    with ops._on(dev):
+        rc = _lib.load().knlp_b200_build_step(
+            context_lens.data_ptr(), query_lens.data_ptr(), block_table.data_ptr(),
+            block_table.stride(0), block_table.shape[1], free_blocks.data_ptr(),
+            free_blocks.numel(), free_head.data_ptr() if free_head is not None else None,
+            S, block_size, num_tokens, starts.data_ptr(), lens.data_ptr(), slots.data_ptr(),
+            positions.data_ptr(), taken.data_ptr(), ops._stream(dev))
+    _lib.check(rc, "knlp_b200_build_step")
+    return StepTables(starts, lens, slots, positions, taken)
+
+
 class AttentionMetadataBuilder:
     """Builds the per-step metadata from the scheduler's common metadata (reference
     FusedInt4AttentionMetadataBuilder.build, :2210-2252): the fields are taken over as they
@@ -103,6 +166,21 @@ class AttentionMetadataBuilder:
             num_actual_tokens=m.num_actual_tokens, max_query_len=m.max_query_len,
             query_start_loc=m.query_start_loc, max_seq_len=m.max_seq_len, seq_lens=m.seq_lens,
             block_table=m.block_table_tensor, slot_mapping=m.slot_mapping)
+
+    def build_from_lengths(self, context_lens: torch.Tensor, query_lens: torch.Tensor,
+                           block_table: torch.Tensor, free_blocks: torch.Tensor, *,
+                           num_tokens: int, max_query_len: int, max_seq_len: int,
+                           free_head: Optional[torch.Tensor] = None
+                           ) -> Tuple[AttentionMetadata, StepTables]:
+        """Metadata of a step whose tables are built here (``build_step``) instead of taken
+        ready-made: the block table is updated in place.  ``num_tokens``, ``max_query_len``,
+        ``max_seq_len``: the host's counts of the step."""
+        t = build_step(context_lens, query_lens, block_table, free_blocks, self.block_size,
+                       num_tokens, free_head=free_head)
+        return AttentionMetadata(
+            num_actual_tokens=num_tokens, max_query_len=max_query_len,
+            query_start_loc=t.query_start_loc, max_seq_len=max_seq_len, seq_lens=t.seq_lens,
+            block_table=block_table, slot_mapping=t.slot_mapping), t
 
 
 class AttentionBackend:
@@ -285,3 +363,36 @@ class PackedKVCache:
         return self.decode(decode_query, meta.block_table, meta.seq_lens,
                            key_cache_fp16=key_cache_fp16, out_dtype=out_dtype,
                            max_seq_len=meta.max_seq_len)
+
+    # ---- several new tokens per sequence (reference forward :2746-2849)
+    def extend(self, query: torch.Tensor, meta: AttentionMetadata,
+               key_cache_fp16: Optional[torch.Tensor] = None, **kw):
+        """Attention of the step's new tokens ([T, Hq, d], already written) over the cache.
+        ``kw``: the keyword arguments of ``ops.extend_attention``."""
+        kw.setdefault("max_query_len", meta.max_query_len)
+        kw.setdefault("max_seq_len", meta.max_seq_len)
+        if self.k_precision == "int4" and self.v_precision != "int4":
+            raise NotImplementedError("K int4 with V int8 is not a mode of the reference")
+        num_blocks, block_size = self.num_blocks, self.block_size
+        if self.k_precision == "fp16" and key_cache_fp16 is not None:
+            if query.dtype != key_cache_fp16.dtype:
+                raise TypeError("the query must have the unquantized K cache's dtype")
+            if tuple(key_cache_fp16.shape[:2]) != (num_blocks, block_size):
+                raise ValueError("the unquantized K cache must have the packed V cache's blocks")
+        return ops.extend_attention(
+            query, self._k_plane(key_cache_fp16), self._v_plane(), num_blocks, meta.block_table,
+            meta.seq_lens, meta.query_start_loc, self.num_kv_heads, self.head_size, block_size,
+            **kw)
+
+    def forward(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+                meta: AttentionMetadata, key_cache_fp16: Optional[torch.Tensor] = None,
+                out_dtype=None) -> torch.Tensor:
+        """One step of any mix of prefill chunks and single tokens (reference forward
+        :2548-2849): write the new tokens, attend.  A step of exactly one new token per
+        sequence is a ``decode_step``; ``meta.seq_lens`` include the new tokens."""
+        S = meta.seq_lens.shape[0]
+        if meta.max_query_len == 1 and meta.num_actual_tokens == S == query.shape[0]:
+            return self.decode_step(query, key, value, meta, key_cache_fp16=key_cache_fp16,
+                                    out_dtype=out_dtype)
+        self.write(key, value, meta.slot_mapping)
+        return self.extend(query, meta, key_cache_fp16=key_cache_fp16, out_dtype=out_dtype)

@@ -3,7 +3,7 @@
 
 #include <atomic>
 
-#include "common.cuh"
+#include "serve.cuh"
 
 using namespace knlp;
 
@@ -12,6 +12,10 @@ namespace {
 bool dtype_ok(int dt) { return dt == KNLP_F32 || dt == KNLP_F16 || dt == KNLP_BF16; }
 
 bool head_dim_ok(int d) { return d == 32 || d == 64 || d == 128 || d == 256; }
+
+}  // namespace
+
+namespace knlp {
 
 // unquantized_k: the plane may also be an fp16 / bf16 K plane (decode only).
 int check_plane(const knlp_kv_plane* p, bool unquantized_k) {
@@ -54,7 +58,7 @@ int sm_count() {
   return n;
 }
 
-}  // namespace
+}  // namespace knlp
 
 extern "C" {
 

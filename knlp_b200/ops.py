@@ -25,6 +25,13 @@ Additions that the reference does not have (keyword-only, all optional):
 so that no device value is read back), ``n_splits``, ``force_generic``, and the
 split-context entry points ``decode_partials`` / ``combine_partials`` used by the
 multi-GPU context shard.
+
+Beside each decode stands the same cache's attention of SEVERAL new tokens per sequence
+(chunked prefill, verification of drafted tokens, mixed batches), which the reference runs
+over an unquantized copy of the cache (:2746-2849):
+
+    fused_int4_extend, kint8_vint4_extend, kint8_vint8_extend, kfp16_vint4_extend,
+    kfp16_vint8_extend, and extend_attention over planes
 """
 
 from __future__ import annotations
@@ -680,3 +687,248 @@ def kfp16_vint8_decode(
     return _decode(query, kp, vp, key_cache_fp16.shape[0], block_table, seq_lens, num_kv_heads,
                    head_size, key_cache_fp16.shape[1], out_dtype, max_seq_len, n_splits,
                    False, False)
+
+
+_extend_ws = {}  # (device index, stream) -> float workspace
+_extend_sizes = {}  # shape -> floats of knlp_b200_extend_workspace
+
+
+def _extend_workspace(dev: torch.device, S: int, T: int, Hq: int, Hkv: int, d: int):
+    """Workspace of ``knlp_b200_extend_attention`` for the current stream, grown on demand
+    and reused by every later call on that stream.  A stream that is being captured gets
+    memory of the graph's own pool: replays do not share it with eager calls."""
+    shape = (dev.index, S, T, Hq, Hkv, d)
+    need = _extend_sizes.get(shape)
+    if need is None:
+        nf = C.c_int64(0)
+        with _on(dev):  # the size depends on the device's SM count
+            rc = _lib.load().knlp_b200_extend_workspace(S, T, Hq, Hkv, d, C.byref(nf))
+        _lib.check(rc, "knlp_b200_extend_workspace")
+        if len(_extend_sizes) >= 4096:
+            _extend_sizes.clear()
+        need = _extend_sizes[shape] = nf.value
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(need, dtype=torch.float32, device=dev)
+    key = (dev.index, _stream(dev))
+    cur = _extend_ws.get(key)
+    if cur is None or cur.numel() < need:
+        cur = _extend_ws[key] = torch.empty(need, dtype=torch.float32, device=dev)
+    return cur
+
+
+def extend_attention(
+    query: torch.Tensor, k_plane: _lib.KvPlane, v_plane: _lib.KvPlane, num_blocks: int,
+    block_table: torch.Tensor, seq_lens: torch.Tensor, query_start_loc: torch.Tensor,
+    num_kv_heads: int, head_size: int, block_size: int, *, causal: bool = True,
+    softmax_scale: Optional[float] = None, max_query_len: Optional[int] = None,
+    max_seq_len: Optional[int] = None, out: Optional[torch.Tensor] = None, out_dtype=None,
+    return_lse: bool = False, force_generic: bool = False,
+):
+    """Attention of several query tokens per sequence over the packed cache
+    (``knlp_b200_extend_attention``).
+
+    query            [T, Hq, d] float16 / bfloat16, the sequences' new tokens one after another
+    query_start_loc  int32 [S + 1], sequence s owns rows [loc[s], loc[s + 1])
+    seq_lens         int32 [S], cached tokens INCLUDING the new ones (already written)
+
+    Query token i of the n of a sequence attends to positions up to ``seq_lens - n + i``;
+    with ``causal=False`` to all ``seq_lens`` tokens.  Rows that attend to nothing give 0
+    (log-sum-exp -inf), rows of no sequence are left as they were in ``out``.
+    ``max_query_len`` / ``max_seq_len``: host-known bounds that size the work only.
+    Returns [T, Hq, d] in ``out_dtype`` (default: the query's), with ``return_lse`` also the
+    fp32 [T, Hq] natural log of the sum of the exponentials."""
+    dev = _need_cuda(query, block_table, seq_lens, query_start_loc, out)
+    if query.dim() != 3:
+        raise ValueError("query must be [num_tokens, num_heads, head_size]")
+    T, Hq, d = query.shape
+    if query.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError("extend attention takes float16 or bfloat16 queries")
+    for t in (block_table, seq_lens, query_start_loc):
+        if t.dtype != torch.int32:
+            raise TypeError("block_table, seq_lens and query_start_loc must be int32")
+    S = seq_lens.shape[0] if seq_lens.dim() == 1 else -1
+    if S < 0 or query_start_loc.shape != (S + 1,) or not seq_lens.is_contiguous() or (
+            not query_start_loc.is_contiguous()):
+        raise ValueError("seq_lens must be [S] and query_start_loc [S + 1], contiguous")
+    if block_table.dim() != 2 or block_table.shape[0] != S or (
+            block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError("block_table must be [S, max_blocks] with contiguous rows")
+    if d != head_size or num_kv_heads <= 0 or Hq % num_kv_heads:
+        raise ValueError("query shape does not match num_kv_heads / head_size")
+    if out is None:
+        out = torch.empty((T, Hq, d), dtype=query.dtype if out_dtype is None else out_dtype,
+                          device=dev)
+    elif out.shape != (T, Hq, d) or not out.is_contiguous():
+        raise ValueError("out must be contiguous [num_tokens, num_heads, head_size]")
+    elif out_dtype is not None and out.dtype != out_dtype:
+        raise ValueError("out and out_dtype disagree")
+    lse = torch.empty((T, Hq), dtype=torch.float32, device=dev) if return_lse else None
+    if T and S:
+        if block_table.shape[1] == 0:
+            raise ValueError("block_table has no columns")
+        ws = _extend_workspace(dev, S, T, Hq, num_kv_heads, d)
+        flags = (0 if causal else _lib.EXTEND_FULL) | (
+            _lib.EXTEND_FORCE_GENERIC if force_generic else 0)
+        with _on(dev):
+            rc = _lib.load().knlp_b200_extend_attention(
+                query.data_ptr(), _dt(query), _stride2(query), C.byref(k_plane),
+                C.byref(v_plane), block_table.data_ptr(), block_table.stride(0),
+                block_table.shape[1], seq_lens.data_ptr(), query_start_loc.data_ptr(),
+                num_blocks, S, T, Hq, num_kv_heads, d, block_size,
+                T if max_query_len is None else max_query_len,
+                block_table.shape[1] * block_size if max_seq_len is None else max_seq_len,
+                d ** -0.5 if softmax_scale is None else softmax_scale,
+                ws.data_ptr(), ws.numel(), out.data_ptr(), _dt(out), d,
+                lse.data_ptr() if lse is not None else None, flags, _stream(dev))
+        _lib.check(rc, "knlp_b200_extend_attention")
+    return (out, lse) if return_lse else out
+
+
+def _cache_shape(codes, scales, zeros, num_kv_heads, head_size, per_byte, what):
+    want = tuple(codes.shape[:2]) + (num_kv_heads,)
+    if codes.dim() != 4 or tuple(codes.shape) != want + (head_size // per_byte,):
+        raise ValueError(f"{what} cache must be [num_blocks, block_size, num_kv_heads, "
+                         f"{head_size // per_byte}]")
+    for t in (scales, zeros):
+        if t is not None and tuple(t.shape) != want + (head_size // GROUP_SIZE,):
+            raise ValueError(f"{what} scales / zeros must be [num_blocks, block_size, "
+                             f"num_kv_heads, {head_size // GROUP_SIZE}]")
+
+
+def _extend(query, k_plane, v_plane, key_cache, value_cache, block_table, seq_lens,
+            query_start_loc, num_kv_heads, head_size, kw):
+    if key_cache.shape[:2] != value_cache.shape[:2]:
+        raise ValueError("the K and V caches differ in num_blocks or block_size")
+    return extend_attention(query, k_plane, v_plane, key_cache.shape[0], block_table, seq_lens,
+                            query_start_loc, num_kv_heads, head_size, key_cache.shape[1], **kw)
+
+
+def fused_int4_extend(
+    query: torch.Tensor,  # [num_tokens, num_heads, head_size] fp16 / bf16
+    key_cache: torch.Tensor,  # [num_blocks, block_size, num_kv_heads, head_size//2]
+    value_cache: torch.Tensor,
+    k_scales: torch.Tensor,  # [num_blocks, block_size, num_kv_heads, head_size//32]
+    v_scales: torch.Tensor,
+    block_table: torch.Tensor,  # [num_seqs, max_num_blocks_per_seq] int32
+    seq_lens: torch.Tensor,  # [num_seqs] int32, with the new tokens
+    query_start_loc: torch.Tensor,  # [num_seqs + 1] int32
+    num_kv_heads: int,
+    head_size: int,
+    k_zeros: Optional[torch.Tensor] = None,
+    v_zeros: Optional[torch.Tensor] = None,
+    asymmetric: bool = False,
+    **kw,
+):
+    """``fused_int4_decode`` for several query tokens per sequence.  ``kw``: the keyword
+    arguments of ``extend_attention``."""
+    _need_cuda(query, key_cache, value_cache, k_scales, v_scales, k_zeros, v_zeros)
+    kp = _plane(key_cache, k_scales, k_zeros if asymmetric else None,
+                _int4_mode(asymmetric, k_zeros))
+    vp = _plane(value_cache, v_scales, v_zeros if asymmetric else None,
+                _int4_mode(asymmetric, v_zeros))
+    _cache_shape(key_cache, k_scales, k_zeros, num_kv_heads, head_size, 2, "K")
+    _cache_shape(value_cache, v_scales, v_zeros, num_kv_heads, head_size, 2, "V")
+    return _extend(query, kp, vp, key_cache, value_cache, block_table, seq_lens,
+                   query_start_loc, num_kv_heads, head_size, kw)
+
+
+def kint8_vint4_extend(
+    query: torch.Tensor,
+    key_cache_int8: torch.Tensor,  # [num_blocks, block_size, kv_heads, head_size] int8
+    value_cache_int4: torch.Tensor,  # [num_blocks, block_size, kv_heads, head_size//2] uint8
+    k_scales: torch.Tensor,
+    v_scales: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    query_start_loc: torch.Tensor,
+    num_kv_heads: int,
+    head_size: int,
+    v_zeros: Optional[torch.Tensor] = None,
+    asymmetric: bool = False,
+    **kw,
+):
+    """``kint8_vint4_decode`` for several query tokens per sequence."""
+    _need_cuda(query, key_cache_int8, value_cache_int4, k_scales, v_scales, v_zeros)
+    kp = _plane(key_cache_int8, k_scales, None, _lib.KV_INT8_G32)
+    vp = _plane(value_cache_int4, v_scales, v_zeros if asymmetric else None,
+                _int4_mode(asymmetric, v_zeros))
+    _cache_shape(key_cache_int8, k_scales, None, num_kv_heads, head_size, 1, "K")
+    _cache_shape(value_cache_int4, v_scales, v_zeros, num_kv_heads, head_size, 2, "V")
+    return _extend(query, kp, vp, key_cache_int8, value_cache_int4, block_table, seq_lens,
+                   query_start_loc, num_kv_heads, head_size, kw)
+
+
+def kint8_vint8_extend(
+    query: torch.Tensor,
+    key_cache_int8: torch.Tensor,  # [num_blocks, block_size, kv_heads, head_size] int8
+    value_cache_int8: torch.Tensor,  # same shape, int8
+    k_scales: torch.Tensor,
+    v_scales: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    query_start_loc: torch.Tensor,
+    num_kv_heads: int,
+    head_size: int,
+    **kw,
+):
+    """``kint8_vint8_decode`` for several query tokens per sequence."""
+    _need_cuda(query, key_cache_int8, value_cache_int8, k_scales, v_scales)
+    kp = _plane(key_cache_int8, k_scales, None, _lib.KV_INT8_G32)
+    vp = _plane(value_cache_int8, v_scales, None, _lib.KV_INT8_G32)
+    _cache_shape(key_cache_int8, k_scales, None, num_kv_heads, head_size, 1, "K")
+    _cache_shape(value_cache_int8, v_scales, None, num_kv_heads, head_size, 1, "V")
+    return _extend(query, kp, vp, key_cache_int8, value_cache_int8, block_table, seq_lens,
+                   query_start_loc, num_kv_heads, head_size, kw)
+
+
+def kfp16_vint4_extend(
+    query: torch.Tensor,  # the K cache's dtype
+    key_cache_fp16: torch.Tensor,  # [num_blocks, block_size, kv_heads, head_size] fp16 / bf16
+    value_cache_int4: torch.Tensor,
+    v_scales: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    query_start_loc: torch.Tensor,
+    num_kv_heads: int,
+    head_size: int,
+    v_zeros: Optional[torch.Tensor] = None,
+    asymmetric: bool = False,
+    **kw,
+):
+    """``kfp16_vint4_decode`` for several query tokens per sequence.  The query must have the
+    K cache's type: the product runs in it."""
+    _need_cuda(query, key_cache_fp16, value_cache_int4, v_scales, v_zeros)
+    if query.dtype != key_cache_fp16.dtype:
+        raise TypeError("the query must have the unquantized K cache's dtype")
+    kp = _fp_plane(key_cache_fp16)
+    vp = _plane(value_cache_int4, v_scales, v_zeros if asymmetric else None,
+                _int4_mode(asymmetric, v_zeros))
+    _cache_shape(key_cache_fp16, None, None, num_kv_heads, head_size, 1, "K")
+    _cache_shape(value_cache_int4, v_scales, v_zeros, num_kv_heads, head_size, 2, "V")
+    return _extend(query, kp, vp, key_cache_fp16, value_cache_int4, block_table, seq_lens,
+                   query_start_loc, num_kv_heads, head_size, kw)
+
+
+def kfp16_vint8_extend(
+    query: torch.Tensor,
+    key_cache_fp16: torch.Tensor,
+    value_cache_int8: torch.Tensor,
+    v_scales: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    query_start_loc: torch.Tensor,
+    num_kv_heads: int,
+    head_size: int,
+    **kw,
+):
+    """``kfp16_vint8_decode`` for several query tokens per sequence.  Query type as
+    ``kfp16_vint4_extend``."""
+    _need_cuda(query, key_cache_fp16, value_cache_int8, v_scales)
+    if query.dtype != key_cache_fp16.dtype:
+        raise TypeError("the query must have the unquantized K cache's dtype")
+    kp = _fp_plane(key_cache_fp16)
+    vp = _plane(value_cache_int8, v_scales, None, _lib.KV_INT8_G32)
+    _cache_shape(key_cache_fp16, None, None, num_kv_heads, head_size, 1, "K")
+    _cache_shape(value_cache_int8, v_scales, None, num_kv_heads, head_size, 1, "V")
+    return _extend(query, kp, vp, key_cache_fp16, value_cache_int8, block_table, seq_lens,
+                   query_start_loc, num_kv_heads, head_size, kw)
