@@ -18,7 +18,7 @@ int knlp_b200_extend_workspace(int n_seqs, int n_tokens, int n_q_heads, int n_kv
   if (n_seqs < 0 || n_tokens < 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads)
     return KNLP_ERR_SHAPE;
   if (head_dim != 32 && head_dim != 64 && head_dim != 128 && head_dim != 256) return KNLP_ERR_SHAPE;
-  *workspace_floats_out = 4;
+  *workspace_floats_out = extend_workspace_floats(n_seqs, n_tokens, n_q_heads, n_kv_heads, head_dim, sm_count());
   return KNLP_OK;
 }
 
@@ -77,6 +77,10 @@ int knlp_b200_extend_attention(const void* query, int q_dtype, const int64_t q_s
   a.out_dtype = out_dtype;
   a.out_row_stride = out_row_stride;
   a.lse = lse;
+  if (!(flags & KNLP_EXTEND_FORCE_GENERIC)) {
+    rc = launch_extend_mma(a, workspace, workspace_floats, sm_count(), static_cast<cudaStream_t>(stream));
+    if (rc <= 0) return rc;  // launched, or failed for good
+  }
   return launch_extend_generic(a, static_cast<cudaStream_t>(stream));
 }
 

@@ -35,12 +35,13 @@ extend_generic_kernel(const ExtendArgs a, int n_rep, int q_groups) {
   const int tok = blockIdx.x;
   const int kvh = blockIdx.y / q_groups, qg = blockIdx.y % q_groups;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int d = a.head_dim, P = a.block_size;
+  const int P = a.block_size;
   const int seq = sequence_of(a.query_start_loc, a.n_seqs, tok);
   if (seq < 0) return;  // a row behind the last sequence stays as it is
-  const int n_new = a.query_start_loc[seq + 1] - a.query_start_loc[seq];
+  int first;
+  const int n_new = extend_rows(a, seq, &first);
   const int len = extend_length(a, seq);
-  const int end = a.causal ? min(len, max(a.seq_lens[seq] - n_new + tok - a.query_start_loc[seq] + 1, 0)) : len;
+  const int end = a.causal ? min(len, max(a.seq_lens[seq] - n_new + tok - first + 1, 0)) : len;
 
   const int h_first = qg * QH;
   float q[QH][EPL], m[QH], l[QH], acc[QH][EPL];

@@ -1,0 +1,868 @@
+// Attention of several query tokens per sequence over the packed cache, on the fifth-generation
+// tensor cores (tcgen05, accumulators in TMEM).
+//
+//   S = Q K^T,  P = exp2(c S - m),  O += P V   per 128 query rows x 128 cached tokens, online
+//   maximum m and sum l per row;  o = O / l.  A query row is one (token, q head) of a kv head's
+//   group, so all q heads of the group share every dequantized K / V tile.
+//
+// What bounds it: from about 64 query rows on, the tensor pipe and the exponentials (a 128 x 128
+// tile costs 2 x 512 tensor cycles at head_dim 128 and 1024 cycles of the SM's 16 ex2 per
+// cycle), below that HBM.  Work items and their split over CTAs: extend_plan.cu.
+//
+// One CTA per SM (it owns all 512 TMEM columns), 16 warps whose registers are dealt out by
+// setmaxnreg (2 x 192 + 88 + 40 = 4 x 128 a lane):
+//   warps 0-3, 4-7   two softmax streams, a thread per query row.  An item of more than 128 rows
+//                    gives each stream its own 128 rows over the same K / V tiles; a smaller
+//                    one gives both streams the same rows and every other tile, and their
+//                    states are merged at the end.  Either way one stream's softmax runs under
+//                    the other's tensor work.
+//   warps 8-11       dequantization: packed rows are staged with cp.async (kStages plane tiles in
+//                    flight), turned into fp16 and written as swizzled tensor-core operands into
+//                    a ring of three tiles (K, V alternating)
+//   warp 12          (13-15 idle) issues the matrix products: S = Q K^T from shared memory, O += P V with P
+//                    read from TMEM, where it overlays S
+//
+// Roundings, all chosen for the tensor cores' fp16 inputs: dequantized K and V, P and (from bf16)
+// Q are rounded to fp16, 2^-11 relative each; products accumulate in fp32, m, l and O are fp32.
+// fp16 is used instead of bf16 because its 2^-11 keeps the result within a bf16 rounding of the
+// 64-bit one, and dequantized values fit its range (codes x an fp16 scale).  An unquantized K
+// plane enters the product as it is stored.
+//
+// INT4 codes leave a 32-bit word as (n0, n4), (n1, n5), (n2, n6), (n3, n7): pairing nibbles four
+// apart takes one AND-OR each.  K keeps that order in the operand and Q is permuted alike; V
+// keeps it too and the output columns are put back in order when they are stored.
+//
+// Every wait on a barrier is bounded: when one runs out, the CTA raises the status word and stops
+// waiting (its results are then wrong, its control flow and addresses stay as they are).
+#pragma once
+
+#include "serve.cuh"
+
+namespace knlp {
+namespace extend {
+
+constexpr int kRows = 128;   // query rows of a stream
+constexpr int kTile = 128;   // cached tokens of a tile
+constexpr int kRing = 3;
+constexpr int kThreads = 16 * 32;
+constexpr int kMiscBytes = 2048;
+constexpr int kBadLists = 4, kBadMost = 15;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+// O is rescaled only when a row's maximum has grown by more than this (in powers of two): P
+// then stays below 2^8, far inside fp16, and most tiles skip the pass over O.
+constexpr float kGrow = 8.0f;
+
+// Modes of a plane inside the kernel: KNLP_KV_* with both unquantized K types as kRaw.
+constexpr int kRaw = KNLP_KV_F16;
+
+// A piece of work: query rows [row0, row0 + rows) of a sequence (a row = token x group head),
+// tiles [tile0, tile1) of its cached tokens, for each of the kv heads in turn.
+struct Entry {
+  int seq, row0, rows, tile0, tile1;
+  int part;  // first row in the partial buffer of kv head 0, or -1: the piece is the whole range
+  int pad0, pad1;
+};
+
+// A tile of rows whose range was cut: pieces lie at part + (piece * heads + head) * rows.
+struct Split {
+  int seq, row0, rows, pieces, part;
+  int first;  // rows x heads of the splits before
+  int pad0, pad1;
+};
+
+struct Plan {
+  int n_entries, n_splits, split_rows, pad;
+};
+
+struct Params {
+  ExtendArgs a;
+  const Plan* plan;
+  const Entry* entries;
+  const Split* splits;
+  float* parts;  // rows of head_dim + 4 floats: o (relative to 2^m), m, l, -, -
+  int* status;
+  int rep;  // q heads per kv head
+};
+
+template <int MODE, int D>
+struct PlaneTile {
+  static constexpr bool kQuant = MODE != kRaw;
+  static constexpr int kRowBytes = MODE == kRaw ? 2 * D : MODE == KNLP_KV_INT8_G32 ? D : D / 2;
+  static constexpr int kChunks = kRowBytes / 16;
+  static constexpr int kScaleBytes = D / 32 * 2;
+  static constexpr int kScaleAt = kTile * kRowBytes;
+  static constexpr int kZeroAt = kScaleAt + (kQuant ? kTile * kScaleBytes : 0);
+  static constexpr int kBytes = kZeroAt + (MODE == KNLP_KV_INT4_ASYM ? kTile * kScaleBytes : 0);
+  // position of a 16-byte chunk in its row, such that eight rows' equal chunks hit all banks
+  static __device__ __forceinline__ int at(int row, int chunk) {
+    constexpr int n = kChunks;
+    const int f = n >= 8 ? row & 7 : (row / (8 / (n < 8 ? n : 8))) & (n - 1);
+    return row * kRowBytes + ((chunk ^ f) << 4);
+  }
+};
+
+template <int KM, int VM, int D>
+struct Layout {
+  static constexpr int kTileBytes = kTile * D * 2;  // one fp16 operand tile, also a Q tile
+  static constexpr int kStageBytes = PlaneTile<KM, D>::kBytes > PlaneTile<VM, D>::kBytes
+                                         ? PlaneTile<KM, D>::kBytes : PlaneTile<VM, D>::kBytes;
+  static constexpr int kRoom = 232448 - 1024 - kMiscBytes - (2 + kRing) * kTileBytes;
+  static constexpr int kStages = kRoom / kStageBytes > 8 ? 8 : kRoom / kStageBytes;
+  static_assert(kStages >= 2, "staging needs two plane tiles");
+  static constexpr int kQ = 0;
+  static constexpr int kRingAt = 2 * kTileBytes;
+  static constexpr int kStageAt = kRingAt + kRing * kTileBytes;
+  static constexpr int kMisc = (kStageAt + kStages * kStageBytes + 127) / 128 * 128;
+  static constexpr int kBytes = kMisc + kMiscBytes + 1024;  // 1024 for the alignment of the base
+};
+
+struct Misc {
+  uint64_t ring_full[kRing], ring_empty[kRing];
+  uint64_t q_full, s_full[2], p_full[2], o_full[2];
+  uint32_t tmem;
+  int abort;
+  float m[kRows], l[kRows];  // second stream's state when both serve the same rows
+  // tokens with a scale or zero-point that is not finite, by item: (token, mask of groups)
+  int bad_count[kBadLists];
+  int2 bad[kBadLists][kBadMost + 1];
+};
+static_assert(sizeof(Misc) <= kMiscBytes, "");
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void mbar_init(uint64_t* b, int n) {
+  asm volatile("mbarrier.init.shared.b64 [%0], %1;" ::"r"(smem_addr(b)), "r"(n) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* b) {
+  asm volatile("mbarrier.arrive.shared.b64 _, [%0];" ::"r"(smem_addr(b)) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint64_t* b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      "selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok) : "r"(smem_addr(b)), "r"(parity) : "memory");
+  return ok;
+}
+// Waits for the phase, at most about two seconds; then, or once another wait of the CTA has
+// given up, returns at once with the CTA's abort flag and the status word set.
+__device__ __forceinline__ void mbar_wait_long(uint64_t* b, uint32_t parity, volatile int* abort,
+                                            int* status) {
+  uint64_t t0, t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
+  while (!mbar_try(b, parity)) {
+    if (*abort) return;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+    if (t - t0 > 2000000000ull) {
+      *abort = 1;
+      atomicExch(status, 1);
+      return;
+    }
+  }
+}
+__device__ __forceinline__ void mbar_wait(uint64_t* b, uint32_t parity, int* abort, int* status) {
+  if (!mbar_try(b, parity)) mbar_wait_long(b, parity, abort, status);
+}
+
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void commit(uint64_t* b) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(b)) : "memory");
+}
+
+// 32 TMEM columns of the warp's 32 lanes, a lane's row per thread.
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+      ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+        "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Shared-memory operand descriptor, 128-byte swizzle.  K-major operands (Q, K): rows of 128
+// bytes in groups of eight, `stride` between groups.  MN-major operand (V as stored, a row per
+// token): `lead` between blocks of 64 columns, `stride` between groups of eight tokens.
+__device__ __forceinline__ uint64_t operand(uint32_t addr, int lead, int stride) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3fff) | static_cast<uint64_t>(lead >> 4) << 16 |
+         static_cast<uint64_t>(stride >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+// Instruction descriptor: fp32 accumulator, fp16 or bf16 inputs, B optionally MN-major.
+__host__ __device__ constexpr uint32_t product(int m, int n, bool bf16, bool b_mn) {
+  return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (b_mn ? 1u << 16 : 0u) |
+         static_cast<uint32_t>(n >> 3) << 17 | static_cast<uint32_t>(m >> 4) << 24;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc)) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc)) : "memory");
+}
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool there) {
+  const int n = there ? BYTES : 0;  // what is not there is filled with zeros
+  if constexpr (BYTES == 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  } else {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
+  }
+}
+
+__device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+__device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+
+// Eight 4-bit codes as fp16 integers, in the order (n0 n4)(n1 n5)(n2 n6)(n3 n7), less 8 when
+// symmetric.  A nibble under the exponent of 1024 is 1024 + n (or + 16 n one nibble up); the
+// subtraction and the scaling by 1/16 are exact.
+template <bool SYM>
+__device__ __forceinline__ void nibbles(uint32_t w, __half2* h) {
+  const __half2 low = as_half2(SYM ? 0xe408e408u : 0xe400e400u);   // -1024 (- 8)
+  const __half2 high = as_half2(SYM ? 0xd480d480u : 0xd400d400u);  // -64 (- 8)
+  const __half2 sixteenth = as_half2(0x2c002c00u);
+  const uint32_t w8 = w >> 8;
+  h[0] = __hadd2(as_half2((w & 0x000f000fu) | 0x64006400u), low);
+  h[1] = __hfma2(as_half2((w & 0x00f000f0u) | 0x64006400u), sixteenth, high);
+  h[2] = __hadd2(as_half2((w8 & 0x000f000fu) | 0x64006400u), low);
+  h[3] = __hfma2(as_half2((w8 & 0x00f000f0u) | 0x64006400u), sixteenth, high);
+}
+
+// One row of a staged plane tile as an operand row: 16-byte chunk c of a 64-column box goes to
+// chunk c ^ (row & 7).  A value is rounded once, from code x scale (+ zero) to fp16.
+template <int MODE, int D>
+__device__ __forceinline__ void dequantize_row(const char* stage, char* tile, int row) {
+  using P = PlaneTile<MODE, D>;
+  auto put = [&](int chunk, uint4 v) {  // chunk: 8 elements of the row
+    *reinterpret_cast<uint4*>(tile + (chunk >> 3) * (kTile * 128) + row * 128 +
+                              (((chunk & 7) ^ (row & 7)) << 4)) = v;
+  };
+  if constexpr (MODE == kRaw) {
+#pragma unroll
+    for (int c = 0; c < P::kChunks; ++c) put(c, *reinterpret_cast<const uint4*>(stage + P::at(row, c)));
+  } else {
+    constexpr int G = D / 32;
+    __half s[G], z[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      s[g] = *reinterpret_cast<const __half*>(stage + P::kScaleAt + row * P::kScaleBytes + 2 * g);
+      if constexpr (MODE == KNLP_KV_INT4_ASYM)
+        z[g] = *reinterpret_cast<const __half*>(stage + P::kZeroAt + row * P::kScaleBytes + 2 * g);
+    }
+#pragma unroll
+    for (int c = 0; c < P::kChunks; ++c) {
+      const uint4 w = *reinterpret_cast<const uint4*>(stage + P::at(row, c));
+      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+      if constexpr (MODE == KNLP_KV_INT8_G32) {  // 16 codes, half a group
+        const __half2 sc = __half2half2(s[c >> 1]);
+        const __half2 bias = as_half2(0xe480e480u);  // -1152: the codes are biased by 128
+        uint32_t o[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t x = u[i] ^ 0x80808080u;
+          o[2 * i] = as_u32(__hmul2(__hadd2(as_half2(__byte_perm(x, 0x64646464u, 0x4140)), bias), sc));
+          o[2 * i + 1] = as_u32(__hmul2(__hadd2(as_half2(__byte_perm(x, 0x64646464u, 0x4342)), bias), sc));
+        }
+        put(2 * c, make_uint4(o[0], o[1], o[2], o[3]));
+        put(2 * c + 1, make_uint4(o[4], o[5], o[6], o[7]));
+      } else {  // 32 codes, one group
+        const __half2 sc = __half2half2(s[c]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          __half2 h[4];
+          nibbles<MODE == KNLP_KV_INT4_SYM>(u[i], h);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if constexpr (MODE == KNLP_KV_INT4_ASYM) h[k] = __hfma2(h[k], sc, __half2half2(z[c]));
+            else h[k] = __hmul2(h[k], sc);
+          }
+          put(4 * c + i, make_uint4(as_u32(h[0]), as_u32(h[1]), as_u32(h[2]), as_u32(h[3])));
+        }
+      }
+    }
+  }
+}
+
+// Groups of a staged V row whose scale or zero-point is not finite.
+template <int MODE, int D>
+__device__ __forceinline__ int not_finite(const char* stage, int row) {
+  using P = PlaneTile<MODE, D>;
+  int mask = 0;
+#pragma unroll
+  for (int g = 0; g < D / 32; ++g) {
+    uint16_t u = *reinterpret_cast<const uint16_t*>(stage + P::kScaleAt + row * P::kScaleBytes + 2 * g);
+    bool bad = (u & 0x7c00) == 0x7c00;
+    if constexpr (MODE == KNLP_KV_INT4_ASYM) {
+      u = *reinterpret_cast<const uint16_t*>(stage + P::kZeroAt + row * P::kScaleBytes + 2 * g);
+      bad |= (u & 0x7c00) == 0x7c00;
+    }
+    mask |= bad << g;
+  }
+  return mask;
+}
+
+// Geometry of an item that every role derives for itself.
+struct Item {
+  Entry e;
+  int head, n, len, ctx, first;  // new tokens, cached tokens, len - n, first query row (token)
+  __device__ Item(const Params& p, int k) {
+    const int heads = p.a.n_kv_heads;
+    const int4* src = reinterpret_cast<const int4*>(p.entries + k / heads);
+    const int4 x = src[0], y = src[1];
+    e = {x.x, x.y, x.z, x.w, y.x, y.y, 0, 0};
+    head = k % heads;
+    n = extend_rows(p.a, e.seq, &first);
+    len = extend_length(p.a, e.seq);
+    ctx = p.a.seq_lens[e.seq] - n;
+  }
+  __device__ int tiles() const { return e.tile1 - e.tile0; }
+  __device__ bool pair() const { return e.rows > kRows; }  // each stream has rows of its own
+  // tiles of stream w
+  __device__ int tiles_of(int w) const { return pair() ? tiles() : (tiles() + 1 - w) / 2; }
+};
+
+template <int KM, int VM, int D>
+__global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_constant__ Params p) {
+  using L = Layout<KM, VM, D>;
+  using KT = PlaneTile<KM, D>;
+  using VT = PlaneTile<VM, D>;
+  extern __shared__ char smem_raw[];
+  char* sm = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+  Misc& mi = *reinterpret_cast<Misc*>(sm + L::kMisc);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const ExtendArgs& a = p.a;
+
+  if (tid == 0) {
+    for (int i = 0; i < kRing; ++i) mbar_init(&mi.ring_full[i], 4), mbar_init(&mi.ring_empty[i], 1);
+    mbar_init(&mi.q_full, 8);
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&mi.s_full[w], 1);
+      mbar_init(&mi.p_full[w], 4);
+      mbar_init(&mi.o_full[w], 1);
+    }
+    mi.abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (tid < kBadLists) mi.bad_count[tid] = 0;
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&mi.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = mi.tmem;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int n_items = p.plan->n_entries * a.n_kv_heads;
+  const bool raw_bf16 = KM == kRaw && a.k.mode == KNLP_KV_BF16;
+#define KNLP_REGISTERS(what, n) asm volatile("setmaxnreg." what ".sync.aligned.u32 " #n ";")
+  auto wait = [&](uint64_t* b, uint32_t phase) { mbar_wait(b, phase & 1, &mi.abort, p.status); };
+
+  if (warp < 8) {
+    // ---------------------------------------------------------------- softmax streams
+    KNLP_REGISTERS("inc", 192);
+    const int w = warp >> 2, row = tid & 127;  // row: of the stream's 128
+    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // the warp's 32 TMEM lanes
+    const uint32_t t_s = tmem + lanes + w * kTile, t_o = tmem + lanes + 256 + w * D;
+    const float c = a.scale * kLog2e;
+    uint32_t n_s = 0, n_o = 0;
+    int serial = 0;
+    for (int k = blockIdx.x; k < n_items; k += gridDim.x) {
+      const Item it(p, k);
+      const int tiles = it.tiles_of(w);
+      const int local = (it.pair() ? w * kRows : 0) + row;  // row of the item
+      const bool valid = local < it.e.rows;
+      const int flat = it.e.row0 + local;
+      const int tok = flat / p.rep;
+      const int limit = !valid ? 0 : a.causal ? max(min(it.ctx + tok + 1, it.len), 0) : it.len;
+      const bool active = (it.pair() ? w * kRows : 0) + (row & ~31) < it.e.rows;  // of the warp
+
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // nobody reads the Q area any more
+      if (it.tiles() && (w == 0 || it.pair())) {
+        // Q tile: D/8 lanes copy a row, 16 bytes each
+        constexpr int kPer = D / 8, kAtOnce = 32 / kPer;
+        char* q = sm + L::kQ + w * L::kTileBytes;
+        const int r0 = (warp & 3) * 32, chunk = lane % kPer;
+#pragma unroll 4
+        for (int i = 0; i < 32; i += kAtOnce) {
+          const int r = r0 + i + lane / kPer;
+          const int lr = (it.pair() ? w * kRows : 0) + r;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (lr < it.e.rows) {
+            const int f = it.e.row0 + lr, t = f / p.rep;
+            const int64_t off = (static_cast<int64_t>(it.first) + t) * a.q_stride[0] +
+                                (static_cast<int64_t>(it.head) * p.rep + (f - t * p.rep)) * a.q_stride[1];
+            v = reinterpret_cast<const uint4*>(static_cast<const char*>(a.q) + 2 * off)[chunk];
+          }
+          if constexpr (KM != kRaw) {
+            if (a.q_dtype == KNLP_BF16) {
+              uint32_t* u = &v.x;
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                u[j] = as_u32(__floats2half2_rn(__uint_as_float(u[j] << 16), __uint_as_float(u[j] & 0xffff0000u)));
+            }
+          }
+          if constexpr (KM == KNLP_KV_INT4_SYM || KM == KNLP_KV_INT4_ASYM) {
+            v = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
+                           __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+          }
+          *reinterpret_cast<uint4*>(q + (chunk >> 3) * (kRows * 128) + r * 128 +
+                                    (((chunk & 7) ^ (r & 7)) << 4)) = v;
+        }
+        fence_smem();
+      }
+      __syncwarp();
+      if (it.tiles() && lane == 0) mbar_arrive(&mi.q_full);
+
+      float m = -INFINITY, l = 0.0f;
+      for (int j = 0; j < tiles; ++j) {
+        const int base = (it.e.tile0 + (it.pair() ? j : 2 * j + w)) * kTile;
+        wait(&mi.s_full[w], n_s++);
+        fence_after();
+        if (active) {
+          float s[kTile];
+#pragma unroll
+          for (int i = 0; i < kTile; i += 32) tmem_ld32(t_s + i, reinterpret_cast<uint32_t*>(s + i));
+          tmem_wait_ld();
+          const int seen = limit - base;
+          if (__any_sync(~0u, seen < kTile)) {
+#pragma unroll
+            for (int i = 0; i < kTile; ++i) s[i] = i < seen ? s[i] : -INFINITY;
+          }
+          float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+          for (int i = 4; i < kTile; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+          const float m_new = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c);
+          if (j == 0) {
+            m = m_new;
+          } else if (__any_sync(~0u, m_new > m + kGrow)) {
+            const float f = m_new == m ? 1.0f : exp2f(m - m_new);
+            m = m_new;
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < D; i += 32) {
+              uint32_t o[32];
+              tmem_ld32(t_o + i, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+              tmem_st32(t_o + i, o);
+            }
+          }
+          const float off = m == -INFINITY ? 0.0f : m;
+          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t pk[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float x0 = fmaf(s[h * 64 + 2 * i], c, -off), x1 = fmaf(s[h * 64 + 2 * i + 1], c, -off);
+              float p0, p1;
+              asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p0) : "f"(x0));
+              asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p1) : "f"(x1));
+              sum[(2 * i) & 3] += p0;
+              sum[(2 * i + 1) & 3] += p1;
+              pk[i] = as_u32(__floats2half2_rn(p0, p1));
+            }
+            tmem_st32(t_s + h * 32, pk);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_wait_st();
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&mi.p_full[w]);
+      }
+
+      // ---- epilogue
+      if (tiles) {
+        wait(&mi.o_full[w], n_o++);
+        fence_after();
+      }
+      float* swap = reinterpret_cast<float*>(sm + L::kQ);  // [column][row] of the second stream
+      const bool merge = !it.pair() && it.tiles_of(1) > 0;
+      if (merge && w == 1) {
+        if (active) {
+#pragma unroll
+          for (int i = 0; i < D; i += 32) {
+            uint32_t o[32];
+            tmem_ld32(t_o + i, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int x = 0; x < 32; ++x) swap[(i + x) * kRows + row] = __uint_as_float(o[x]);
+          }
+          mi.m[row] = m;
+          mi.l[row] = l;
+        }
+        fence_before();
+      }
+      if (merge) asm volatile("bar.sync 2, 256;" ::: "memory");
+      if (active && (w == 0 || it.pair())) {
+        float f0 = 1.0f, f1 = 0.0f;
+        if (merge) {
+          const float m1 = mi.m[row], mm = fmaxf(m, m1);
+          f0 = m == mm ? 1.0f : exp2f(m - mm);
+          f1 = m1 == mm ? 1.0f : exp2f(m1 - mm);
+          l = l * f0 + mi.l[row] * f1;
+          m = mm;
+        }
+        const bool direct = it.e.part < 0;
+        const float inv = !direct ? 1.0f : l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
+        const int bad = mi.bad_count[serial % kBadLists];
+        const int h = flat - tok * p.rep;
+        const int64_t out_row = (static_cast<int64_t>(it.first) + tok) * a.n_q_heads + it.head * p.rep + h;
+        float* part = direct ? nullptr
+                             : p.parts + (static_cast<int64_t>(it.e.part) + static_cast<int64_t>(it.head) * it.e.rows + local) * (D + 4);
+#pragma unroll
+        for (int i = 0; i < D; i += 32) {
+          float o[32];
+          if (tiles) {
+            tmem_ld32(t_o + i, reinterpret_cast<uint32_t*>(o));
+            tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int x = 0; x < 32; ++x) o[x] = 0.0f;
+          }
+#pragma unroll
+          for (int x = 0; x < 32; ++x) {
+            if (merge) o[x] = o[x] * f0 + swap[(i + x) * kRows + row] * f1;
+            o[x] *= inv;
+          }
+          if (bad) {  // never in a healthy cache
+            for (int b = 0; b < min(bad, kBadMost + 1); ++b) {
+              const int2 t = mi.bad[serial % kBadLists][b];
+              if (limit > t.x && (t.y >> (i / 32) & 1)) {
+#pragma unroll
+                for (int x = 0; x < 32; ++x) o[x] = NAN;
+              }
+            }
+          }
+          if (!valid) continue;
+          float v[32];  // in the order of the head dimension
+#pragma unroll
+          for (int x = 0; x < 32; ++x) {
+            constexpr bool kPaired = VM == KNLP_KV_INT4_SYM || VM == KNLP_KV_INT4_ASYM;
+            v[x] = o[kPaired ? (x & ~7) + 2 * (x & 3) + ((x >> 2) & 1) : x];
+          }
+          if (!direct) {
+#pragma unroll
+            for (int x = 0; x < 32; x += 4)
+              *reinterpret_cast<float4*>(part + i + x) = make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+          } else if (a.out_dtype == KNLP_F32) {
+            float* dst = static_cast<float*>(a.out) + out_row * a.out_row_stride + i;
+#pragma unroll
+            for (int x = 0; x < 32; x += 4)
+              *reinterpret_cast<float4*>(dst + x) = make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+          } else {
+            uint16_t* dst = static_cast<uint16_t*>(a.out) + out_row * a.out_row_stride + i;
+            uint32_t u[16];
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+              if (a.out_dtype == KNLP_F16) {
+                u[x] = as_u32(__floats2half2_rn(v[2 * x], v[2 * x + 1]));
+              } else {
+                const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * x], v[2 * x + 1]);
+                u[x] = *reinterpret_cast<const uint32_t*>(&b);
+              }
+            }
+#pragma unroll
+            for (int x = 0; x < 16; x += 4)
+              *reinterpret_cast<uint4*>(dst + 2 * x) = make_uint4(u[x], u[x + 1], u[x + 2], u[x + 3]);
+          }
+        }
+        if (valid) {
+          if (!direct) {
+            part[D] = m;
+            part[D + 1] = l;
+          } else if (a.lse) {
+            a.lse[out_row] = l == 0.0f ? -INFINITY : kLn2 * (m + log2f(l));
+          }
+        }
+      }
+      fence_before();
+      serial += it.tiles() > 0;
+    }
+  } else if (warp < 12) {
+    // ---------------------------------------------------------------- staging, dequantization
+    // Plane tiles in the order K0 V0 K1 V1 ..., item after item.  A warp stages and converts rows
+    // 32 w .. 32 w + 31 of every tile, a lane converts one row; only lanes of the same warp
+    // read what a lane has copied.
+    KNLP_REGISTERS("dec", 88);
+    const int w = warp - 8, row = w * 32 + lane;
+    struct Cursor {  // next plane tile to copy
+      int k, tile, tile1, len, head;
+      const int32_t* table;
+      int block, off;
+    } cur;
+    auto open = [&](Cursor& x, int k) {  // first tile of item k or of the first later one that has any
+      for (; k < n_items; k += gridDim.x) {
+        const Item it(p, k);
+        if (it.tiles() == 0) continue;
+        x.tile = it.e.tile0, x.tile1 = it.e.tile1, x.len = it.len, x.head = it.head;
+        x.table = a.block_table + it.e.seq * a.bt_stride;
+        break;
+      }
+      x.k = k;
+    };
+    open(cur, blockIdx.x);
+    uint32_t copied = 0;
+    auto copy_plane = [&](const Plane& pl, auto tag, char* stage, bool there) {
+      using T = decltype(tag);
+      const char* row_base = reinterpret_cast<const char*>(pl.codes) + cur.head * pl.cs[2];
+      constexpr int n = T::kChunks, rows_at_once = 32 / n;
+      const int chunk = lane % n;
+#pragma unroll
+      for (int i = 0; i < 32; i += rows_at_once) {
+        const int r = i + lane / n;
+        const int block = __shfl_sync(~0u, cur.block, r), off = __shfl_sync(~0u, cur.off, r);
+        const char* src = row_base + block * pl.cs[0] + off * pl.cs[1] + chunk * 16;
+        const bool ok = __shfl_sync(~0u, there, r);
+        copy_async<16>(smem_addr(stage + T::at(w * 32 + r, chunk)), ok ? src : row_base, ok);
+      }
+      if constexpr (T::kQuant) {
+        const int64_t so = cur.block * pl.ss[0] + cur.off * pl.ss[1] + cur.head * pl.ss[2];
+        copy_async<T::kScaleBytes>(smem_addr(stage + T::kScaleAt + row * T::kScaleBytes), pl.scales + (there ? so : 0), there);
+        if constexpr (T::kBytes > T::kZeroAt) {
+          const int64_t zo = cur.block * pl.zs[0] + cur.off * pl.zs[1] + cur.head * pl.zs[2];
+          copy_async<T::kScaleBytes>(smem_addr(stage + T::kZeroAt + row * T::kScaleBytes), pl.zeros + (there ? zo : 0), there);
+        }
+      }
+    };
+    auto copy_next = [&]() {
+      if (cur.k < n_items) {
+        char* stage = sm + L::kStageAt + copied % L::kStages * L::kStageBytes;
+        const int t = cur.tile * kTile + row;
+        const bool there = t < cur.len;
+        if (copied & 1) {
+          copy_plane(a.v, VT{}, stage, there);
+          if (++cur.tile == cur.tile1) open(cur, cur.k + gridDim.x);
+        } else {
+          const int e = t / a.block_size;
+          int64_t block = there ? cur.table[e] : 0;
+          block = block < 0 ? 0 : block >= a.num_blocks ? a.num_blocks - 1 : block;
+          cur.block = static_cast<int>(block);
+          cur.off = t - e * a.block_size;
+          copy_plane(a.k, KT{}, stage, there);
+        }
+        ++copied;
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    for (int i = 0; i < L::kStages - 1; ++i) copy_next();
+    uint32_t done = 0;
+    int serial = 0;
+    for (int k = blockIdx.x; k < n_items; k += gridDim.x) {
+      const Item it(p, k);
+      if (it.tiles() == 0) continue;
+      if (row == 0) {
+        mi.bad_count[serial % kBadLists] = 0;
+        mi.bad[serial % kBadLists][kBadMost] = make_int2(0x7fffffff, 0);
+      }
+      asm volatile("bar.sync 3, 128;" ::: "memory");
+      for (int j = 0; j < it.tiles(); ++j) {
+#pragma unroll
+        for (int plane = 0; plane < 2; ++plane, ++done) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 2) : "memory");
+          __syncwarp();
+          char* stage = sm + L::kStageAt + done % L::kStages * L::kStageBytes;
+          char* tile = sm + L::kRingAt + done % kRing * L::kTileBytes;
+          wait(&mi.ring_empty[done % kRing], done / kRing + 1);
+          if (plane == 0) {
+            dequantize_row<KM, D>(stage, tile, row);
+          } else {
+            // A value that is not finite would reach rows that do not attend to its token (as
+            // 0 x NaN): such groups are zeroed here and noted, and the rows that do attend
+            // to the token are made NaN at the end.
+            const int bad = not_finite<VM, D>(stage, row);
+            if (bad) {
+              char* sc = stage + VT::kScaleAt + row * VT::kScaleBytes;
+              for (int g = 0; g < D / 32; ++g) {
+                if (!(bad >> g & 1)) continue;
+                *reinterpret_cast<uint16_t*>(sc + 2 * g) = 0;
+                if constexpr (VT::kBytes > VT::kZeroAt)
+                  *reinterpret_cast<uint16_t*>(stage + VT::kZeroAt + row * VT::kScaleBytes + 2 * g) = 0;
+              }
+              const int token = (it.e.tile0 + j) * kTile + row;
+              const int at = atomicAdd(&mi.bad_count[serial % kBadLists], 1);
+              int2* list = mi.bad[serial % kBadLists];
+              if (at < kBadMost) {
+                list[at] = make_int2(token, bad);
+              } else {  // more than the list holds: from the first of them on, all their groups
+                atomicMin(&list[kBadMost].x, token);
+                atomicOr(&list[kBadMost].y, bad);
+              }
+            }
+            dequantize_row<VM, D>(stage, tile, row);
+          }
+          fence_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&mi.ring_full[done % kRing]);
+          copy_next();
+        }
+      }
+      ++serial;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else {
+    // ---------------------------------------------------------------- matrix products
+    KNLP_REGISTERS("dec", 40);
+    if (warp == 12 && lane == 0) {
+      const uint32_t q_at = smem_addr(sm + L::kQ), ring_at = smem_addr(sm + L::kRingAt);
+      const uint32_t idesc_s = product(kRows, kTile, raw_bf16, false);
+      const uint32_t idesc_o = product(kRows, D, false, true);
+      uint32_t used = 0, n_q = 0, n_p[2] = {0, 0};
+      auto scores = [&](int w, int qt, uint32_t slot) {  // S of stream w = Q tile qt x K tile
+        const uint32_t q = q_at + qt * L::kTileBytes, kk = ring_at + slot * L::kTileBytes;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          const uint32_t off = (i >> 2) * (kTile * 128) + (i & 3) * 32;
+          mma_ss(tmem + w * kTile, operand(q + off, 16, 1024), operand(kk + off, 16, 1024), idesc_s, i > 0);
+        }
+      };
+      auto values = [&](int w, uint32_t slot, bool acc) {  // O of stream w += P x V tile
+        const uint32_t v = ring_at + slot * L::kTileBytes;
+#pragma unroll
+        for (int i = 0; i < kTile / 16; ++i)
+          mma_ts(tmem + 256 + w * D, tmem + w * kTile + i * 8, operand(v + i * 2048, kTile * 128, 1024), idesc_o, acc || i > 0);
+      };
+      auto ready = [&](uint32_t x) {  // plane tile x of the ring
+        wait(&mi.ring_full[x % kRing], x / kRing);
+        fence_after();
+        return x % kRing;
+      };
+      auto probs = [&](int w) {
+        wait(&mi.p_full[w], n_p[w]++);
+        fence_after();
+      };
+      for (int k = blockIdx.x; k < n_items; k += gridDim.x) {
+        const Item it(p, k);
+        const int n = it.tiles();
+        if (n == 0) continue;
+        wait(&mi.q_full, n_q++);
+        fence_after();
+        if (it.pair()) {
+          uint32_t slot = ready(used);
+          scores(0, 0, slot), commit(&mi.s_full[0]);
+          scores(1, 1, slot), commit(&mi.s_full[1]);
+          commit(&mi.ring_empty[slot]);
+          for (int j = 0; j < n; ++j, used += 2) {
+            const bool more = j + 1 < n;
+            const uint32_t v = ready(used + 1);
+            probs(0);
+            values(0, v, j > 0);
+            if (more) {
+              slot = ready(used + 2);
+              scores(0, 0, slot), commit(&mi.s_full[0]);
+            } else {
+              commit(&mi.o_full[0]);
+            }
+            probs(1);
+            values(1, v, j > 0);
+            commit(&mi.ring_empty[v]);
+            if (more) {
+              scores(1, 1, slot), commit(&mi.s_full[1]);
+              commit(&mi.ring_empty[slot]);
+            } else {
+              commit(&mi.o_full[1]);
+            }
+          }
+        } else {
+          for (int w = 0; w < 2 && w < n; ++w) {
+            const uint32_t slot = ready(used + 2 * w);
+            scores(w, 0, slot), commit(&mi.s_full[w]), commit(&mi.ring_empty[slot]);
+          }
+          for (int j = 0; j < n; ++j, used += 2) {
+            const int w = j & 1;
+            const uint32_t v = ready(used + 1);
+            probs(w);
+            values(w, v, j > 1);
+            commit(&mi.ring_empty[v]);
+            if (j + 2 < n) {
+              const uint32_t slot = ready(used + 4);
+              scores(w, 0, slot), commit(&mi.s_full[w]), commit(&mi.ring_empty[slot]);
+            } else {
+              commit(&mi.o_full[w]);
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 12)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+// One pair of plane modes, both head dimensions.
+template <int KM, int VM>
+int launch_extend_pair(const Params& p, int grid, cudaStream_t st);
+
+template <int KM, int VM, int D>
+int launch_extend_one(const Params& p, int grid, cudaStream_t st) {
+  using L = Layout<KM, VM, D>;
+  auto* fn = extend_mma_kernel<KM, VM, D>;
+  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes) != cudaSuccess) {
+    cudaGetLastError();
+    return KNLP_ERR_NO_DEVICE;
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = L::kBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, fn, p) != cudaSuccess) {
+    cudaGetLastError();
+    return KNLP_ERR_LAUNCH;
+  }
+  return KNLP_OK;
+}
+
+#undef KNLP_REGISTERS
+
+#define KNLP_EXTEND_PAIR(KM, VM)                                                   \
+  namespace knlp {                                                                 \
+  namespace extend {                                                               \
+  template <>                                                                      \
+  int launch_extend_pair<KM, VM>(const Params& p, int grid, cudaStream_t st) {     \
+    return p.a.head_dim == 64 ? launch_extend_one<KM, VM, 64>(p, grid, st)         \
+                              : launch_extend_one<KM, VM, 128>(p, grid, st);       \
+  }                                                                                \
+  }                                                                                \
+  }
+
+}  // namespace extend
+}  // namespace knlp

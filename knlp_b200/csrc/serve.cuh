@@ -37,6 +37,23 @@ __device__ __forceinline__ int extend_length(const ExtendArgs& a, int seq) {
   return n < most ? n : static_cast<int>(most);
 }
 
+// New tokens of a sequence and its first query row, kept inside the query whatever the offsets.
+__device__ __forceinline__ int extend_rows(const ExtendArgs& a, int seq, int* first) {
+  const int lo = min(max(a.query_start_loc[seq], 0), a.n_tokens);
+  const int hi = min(max(a.query_start_loc[seq + 1], 0), a.n_tokens);
+  *first = lo;
+  return max(hi - lo, 0);
+}
+
+// Tensor-core kernel (extend_plan.cu, extend_mma.cuh).  Returns KNLP_OK, 1 if the layout is not
+// one it addresses (nothing launched), < 0 on error.
+int launch_extend_mma(const ExtendArgs& a, float* ws, int64_t ws_floats, int n_sms,
+                      cudaStream_t st);
+int64_t extend_workspace_floats(int n_seqs, int n_tokens, int n_q_heads, int n_kv_heads,
+                                int head_dim, int n_sms);
+// Device-side status word shared by the kernels with bounded waits (decode_mma.cu).
+int* decode_status_ptr();
+
 int launch_extend_generic(const ExtendArgs& a, cudaStream_t st);
 
 int launch_step_tables(const int32_t* ctx, const int32_t* fresh_tokens, int32_t* table,

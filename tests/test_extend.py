@@ -111,9 +111,10 @@ class Batch:
     def reference(self, causal=True, scale=None):
         """(o, lse, bound of o, bound of lse) in 64 bits, rows [T, hq].
 
-        The bound: K and V are rounded to fp16 after dequantization and P to fp16 (each within
-        2^-11 of its value, P also within 2^-25), products are summed in fp32, exponentials
-        are good to 2^-20.  A score is then off by at most e = scale sum|q k| (2^-11 + d 2^-24),
+        The bound: K and V are rounded to fp16 after dequantization, a bf16 Q below 2^-14 and P
+        to fp16 (each within 2^-11 of its value or 2^-25), products are summed in fp32,
+        exponentials are good to 2^-20.  A score is then off by at most
+        e = scale sum (|q k| (2^-11 + d 2^-24) + |k| 2^-25 + |q| 2^-25),
         which changes every normalized weight by at most a factor exp(2e); so o is within
         (exp(2e) - 1 + 2 * 2^-11 + 2^-18) sum p |v| + n 2^-25 max|v|, and lse within e + 2^-18."""
         dev = self.query.device
@@ -135,7 +136,8 @@ class Batch:
             v = vv[blocks].flatten(0, 1)[:n].repeat_interleave(rep, 1)
             q = self.query[a:b].double()
             w = torch.einsum("qhd,khd->hqk", q, k) * scale
-            e = torch.einsum("qhd,khd->hqk", q.abs(), k.abs()) * scale * (2.0 ** -11 + self.d * 2.0 ** -24)
+            e = torch.einsum("qhd,khd->hqk", q.abs(), k.abs()) * (2.0 ** -11 + self.d * 2.0 ** -24)
+            e = scale * (e + 2.0 ** -25 * (k.abs().sum(-1).t()[:, None] + q.abs().sum(-1).t()[..., None]))
             if causal:
                 last = lens[s] - (b - a) + torch.arange(b - a, device=dev)
                 off = torch.arange(n, device=dev)[None] > last[:, None]
@@ -146,7 +148,7 @@ class Batch:
             o[a:b] = torch.einsum("hqk,khd->qhd", p, v)
             lse[a:b] = ls.t()
             bo[a:b] = (torch.expm1(2 * worst) + 2 * 2.0 ** -11 + 2.0 ** -18).t()[..., None] * (
-                torch.einsum("hqk,khd->qhd", p, v.abs())) + n * 2.0 ** -25 * v.abs().amax()
+                torch.einsum("hqk,khd->qhd", p, v.abs())) + n * 2.0 ** -25 * (1 + v.abs().amax())
             bl[a:b] = worst.t() + 2.0 ** -18 * (1 + torch.where(ls.isinf(), 0, ls).abs().t())
         return o, lse, bo, bl
 
@@ -292,6 +294,34 @@ def test_bad_table_entries_do_not_fault(generic, cuda_device):
     b.table[0, 2], b.table[1, 0] = 1 << 30, -(1 << 30)
     b.run(force_generic=generic)
     torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("generic", GENERIC)
+@pytest.mark.parametrize("mode,many", [("int4_asym", False), ("k8v8", False), ("int4_sym", False),
+                                       ("int4_asym", True)])
+def test_values_that_are_not_finite_reach_only_the_rows_that_see_them(mode, many, generic, cuda_device):
+    """An overflowed scale or zero-point of V belongs to the rows that attend to its token: rows
+    before it (the mask leaves 0 x NaN there) are as if it were not."""
+    b = Batch(cuda_device, [40, 300], [200, 5], 8, 2, 128, mode, seed=17)
+    o, _, bo, _ = b.reference()
+    T, at = b.T, 40 + 90  # the token at position 130 of the first sequence, its kv head 1, group 2
+    tokens = range(at, at + 40) if many else (at,)
+    for t in tokens:
+        blk, off = int(b.table[0, t // 16]), t % 16
+        b.vs[blk, off, 1, 2] = math.inf
+        if b.vz is not None:
+            b.vz[blk, off, 1, 2] = -math.inf
+    if mode == "int4_sym":
+        b.vs[blk, off, 1, 2] = math.nan  # inf x code would be inf or NaN by the code
+    elif mode == "k8v8":
+        b.vs[blk, off, 1, 2] = math.nan
+    r = b.run(force_generic=generic, out_dtype=torch.float32).double()
+    see = torch.zeros(T, 8, 128, dtype=torch.bool, device=cuda_device)
+    see[90:200, 4:, 64:96] = True
+    fine = (r - o).abs() <= bo + 2.0 ** -23 * o.abs()
+    assert torch.isnan(r[see]).all()
+    assert fine[~see].all()
 
 
 @pytest.mark.gpu
