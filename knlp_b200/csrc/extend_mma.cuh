@@ -9,18 +9,18 @@
 // tile costs 2 x 512 tensor cycles at head_dim 128 and 1024 cycles of the SM's 16 ex2 per
 // cycle), below that HBM.  Work items and their split over CTAs: extend_plan.cu.
 //
-// One CTA per SM (it owns all 512 TMEM columns), 16 warps whose registers are dealt out by
-// setmaxnreg (2 x 192 + 88 + 40 = 4 x 128 a lane):
+// One CTA per SM (it owns all 512 TMEM columns), 20 warps whose registers are dealt out by
+// setmaxnreg (2 x 136 + 2 x 80 + 48 = 5 x 96 a lane):
 //   warps 0-3, 4-7   two softmax streams, a thread per query row.  An item of more than 128 rows
 //                    gives each stream its own 128 rows over the same K / V tiles; a smaller
 //                    one gives both streams the same rows and every other tile, and their
 //                    states are merged at the end.  Either way one stream's softmax runs under
 //                    the other's tensor work.
-//   warps 8-11       dequantization: packed rows are staged with cp.async (kStages plane tiles in
-//                    flight), turned into fp16 and written as swizzled tensor-core operands into
-//                    a ring of three tiles (K, V alternating)
-//   warp 12          (13-15 idle) issues the matrix products: S = Q K^T from shared memory, O += P V with P
-//                    read from TMEM, where it overlays S
+//   warps 8-11 (K),  dequantization: packed rows are staged with cp.async a few tiles ahead, turned
+//   12-15 (V)        into fp16 and written as swizzled tensor-core operands into a ring of three
+//                    tiles (K, V alternating).  An unquantized K tile is copied into the ring
+//   warp 16          (17-19 idle) issues the matrix products: S = Q K^T from shared memory,
+//                    O += P V with P read from TMEM, where it overlays S
 //
 // Roundings, all chosen for the tensor cores' fp16 inputs: dequantized K and V, P and (from bf16)
 // Q are rounded to fp16, 2^-11 relative each; products accumulate in fp32, m, l and O are fp32.
@@ -44,7 +44,7 @@ namespace extend {
 constexpr int kRows = 128;   // query rows of a stream
 constexpr int kTile = 128;   // cached tokens of a tile
 constexpr int kRing = 3;
-constexpr int kThreads = 16 * 32;
+constexpr int kThreads = 20 * 32;
 constexpr int kMiscBytes = 2048;
 constexpr int kBadLists = 4, kBadMost = 15;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -82,7 +82,8 @@ struct Params {
   const Split* splits;
   float* parts;  // rows of head_dim + 4 floats: o (relative to 2^m), m, l, -, -
   int* status;
-  int rep;  // q heads per kv head
+  int rep;          // q heads per kv head
+  int block_shift;  // log2 of the block size, -1 if it is no power of two
 };
 
 template <int MODE, int D>
@@ -105,20 +106,25 @@ struct PlaneTile {
 template <int KM, int VM, int D>
 struct Layout {
   static constexpr int kTileBytes = kTile * D * 2;  // one fp16 operand tile, also a Q tile
-  static constexpr int kStageBytes = PlaneTile<KM, D>::kBytes > PlaneTile<VM, D>::kBytes
-                                         ? PlaneTile<KM, D>::kBytes : PlaneTile<VM, D>::kBytes;
   static constexpr int kRoom = 232448 - 1024 - kMiscBytes - (2 + kRing) * kTileBytes;
-  static constexpr int kStages = kRoom / kStageBytes > 8 ? 8 : kRoom / kStageBytes;
-  static_assert(kStages >= 2, "staging needs two plane tiles");
+  static constexpr int kK = KM == kRaw ? 0 : PlaneTile<KM, D>::kBytes, kV = PlaneTile<VM, D>::kBytes;
+  static constexpr int kBoth = kRoom / (kK + kV) < 5 ? kRoom / (kK + kV) : 5;
+  static constexpr int kLeft = kRoom - kBoth * (kK + kV);
+  static constexpr int kStagesK = kK == 0 ? 0 : kBoth + (kBoth < 5 && kLeft >= kK);
+  static constexpr int kStagesV = kBoth + (kBoth < 5 && kLeft - (kStagesK - kBoth) * kK >= kV && kK != 0);
+  static_assert(kBoth >= 1, "a plane tile of each kind has to fit");
   static constexpr int kQ = 0;
   static constexpr int kRingAt = 2 * kTileBytes;
-  static constexpr int kStageAt = kRingAt + kRing * kTileBytes;
-  static constexpr int kMisc = (kStageAt + kStages * kStageBytes + 127) / 128 * 128;
+  static constexpr int kStageK = kRingAt + kRing * kTileBytes;
+  static constexpr int kStageV = kStageK + kStagesK * kK;
+  static constexpr int kMisc = (kStageV + kStagesV * kV + 127) / 128 * 128;
   static constexpr int kBytes = kMisc + kMiscBytes + 1024;  // 1024 for the alignment of the base
+  static_assert(kBytes <= 232448, "shared memory of an SM");
 };
 
 struct Misc {
-  uint64_t ring_full[kRing], ring_empty[kRing];
+  uint64_t ring_full[kRing];
+  uint64_t ring_empty[2][kRing];  // a K tile, a V tile in the slot has been used
   uint64_t q_full, s_full[2], p_full[2], o_full[2];
   uint32_t tmem;
   int abort;
@@ -225,6 +231,13 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc)) : "memory");
 }
 
+// One lane of the converged warp.
+__device__ __forceinline__ bool elect() {
+  uint32_t e;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(e));
+  return e;
+}
+
 template <int BYTES>
 __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool there) {
   const int n = there ? BYTES : 0;  // what is not there is filled with zeros
@@ -237,6 +250,31 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool t
 
 __device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+
+// Two fp32 lanes in one instruction, and the maximum of three.
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
 // Eight 4-bit codes as fp16 integers, in the order (n0 n4)(n1 n5)(n2 n6)(n3 n7), less 8 when
 // symmetric.  A nibble under the exponent of 1024 is 1024 + n (or + 16 n one nibble up); the
@@ -262,24 +300,22 @@ __device__ __forceinline__ void dequantize_row(const char* stage, char* tile, in
     *reinterpret_cast<uint4*>(tile + (chunk >> 3) * (kTile * 128) + row * 128 +
                               (((chunk & 7) ^ (row & 7)) << 4)) = v;
   };
-  if constexpr (MODE == kRaw) {
-#pragma unroll
-    for (int c = 0; c < P::kChunks; ++c) put(c, *reinterpret_cast<const uint4*>(stage + P::at(row, c)));
-  } else {
+  {
     constexpr int G = D / 32;
-    __half s[G], z[G];
+    __half2 s[G / 2], z[G / 2];
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      s[g] = *reinterpret_cast<const __half*>(stage + P::kScaleAt + row * P::kScaleBytes + 2 * g);
+    for (int g = 0; g < G / 2; ++g) {
+      s[g] = reinterpret_cast<const __half2*>(stage + P::kScaleAt + row * P::kScaleBytes)[g];
       if constexpr (MODE == KNLP_KV_INT4_ASYM)
-        z[g] = *reinterpret_cast<const __half*>(stage + P::kZeroAt + row * P::kScaleBytes + 2 * g);
+        z[g] = reinterpret_cast<const __half2*>(stage + P::kZeroAt + row * P::kScaleBytes)[g];
     }
+    auto pick = [](const __half2* v, int g) { return g & 1 ? __high2half2(v[g >> 1]) : __low2half2(v[g >> 1]); };
 #pragma unroll
     for (int c = 0; c < P::kChunks; ++c) {
       const uint4 w = *reinterpret_cast<const uint4*>(stage + P::at(row, c));
       const uint32_t u[4] = {w.x, w.y, w.z, w.w};
       if constexpr (MODE == KNLP_KV_INT8_G32) {  // 16 codes, half a group
-        const __half2 sc = __half2half2(s[c >> 1]);
+        const __half2 sc = pick(s, c >> 1);
         const __half2 bias = as_half2(0xe480e480u);  // -1152: the codes are biased by 128
         uint32_t o[8];
 #pragma unroll
@@ -291,14 +327,16 @@ __device__ __forceinline__ void dequantize_row(const char* stage, char* tile, in
         put(2 * c, make_uint4(o[0], o[1], o[2], o[3]));
         put(2 * c + 1, make_uint4(o[4], o[5], o[6], o[7]));
       } else {  // 32 codes, one group
-        const __half2 sc = __half2half2(s[c]);
+        const __half2 sc = pick(s, c);
+        __half2 zc;
+        if constexpr (MODE == KNLP_KV_INT4_ASYM) zc = pick(z, c);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           __half2 h[4];
           nibbles<MODE == KNLP_KV_INT4_SYM>(u[i], h);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            if constexpr (MODE == KNLP_KV_INT4_ASYM) h[k] = __hfma2(h[k], sc, __half2half2(z[c]));
+            if constexpr (MODE == KNLP_KV_INT4_ASYM) h[k] = __hfma2(h[k], sc, zc);
             else h[k] = __hmul2(h[k], sc);
           }
           put(4 * c + i, make_uint4(as_u32(h[0]), as_u32(h[1]), as_u32(h[2]), as_u32(h[3])));
@@ -308,7 +346,21 @@ __device__ __forceinline__ void dequantize_row(const char* stage, char* tile, in
   }
 }
 
-// Groups of a staged V row whose scale or zero-point is not finite.
+// Whether a scale or zero-point of a staged V row is not finite (x * 0 is then NaN).
+template <int MODE, int D>
+__device__ __forceinline__ bool any_not_finite(const char* stage, int row) {
+  using P = PlaneTile<MODE, D>;
+  __half2 t = __float2half2_rn(0.0f);
+#pragma unroll
+  for (int g = 0; g < D / 64; ++g) {
+    t = __hfma2(reinterpret_cast<const __half2*>(stage + P::kScaleAt + row * P::kScaleBytes)[g], __float2half2_rn(0.0f), t);
+    if constexpr (MODE == KNLP_KV_INT4_ASYM)
+      t = __hfma2(reinterpret_cast<const __half2*>(stage + P::kZeroAt + row * P::kScaleBytes)[g], __float2half2_rn(0.0f), t);
+  }
+  return !__hbeq2(t, t);
+}
+
+// The groups that are concerned, as a mask.
 template <int MODE, int D>
 __device__ __forceinline__ int not_finite(const char* stage, int row) {
   using P = PlaneTile<MODE, D>;
@@ -346,11 +398,153 @@ struct Item {
   __device__ int tiles_of(int w) const { return pair() ? tiles() : (tiles() + 1 - w) / 2; }
 };
 
+// One plane's tiles (SIDE 0: K, 1: V), item after item, by a warpgroup: warp w copies and converts
+// rows 32 w .. 32 w + 31 of every tile, a lane converts one row, and only lanes of the same
+// warp read what a lane has copied.  The block of a row is looked up a tile before it is needed.
+template <class L, int MODE, int D, int SIDE>
+__device__ __forceinline__ void produce(const Params& p, char* sm, Misc& mi, int n_items, int w,
+                                        int lane) {
+  using T = PlaneTile<MODE, D>;
+  constexpr int kStages = SIDE ? L::kStagesV : L::kStagesK;
+  constexpr int kAhead = kStages ? kStages : 1;
+  const ExtendArgs& a = p.a;
+  const Plane& pl = SIDE ? a.v : a.k;
+  char* const stages = sm + (SIDE ? L::kStageV : L::kStageK);
+  const int row = w * 32 + lane;
+
+  // the next tile to copy: its row of this lane
+  int k = blockIdx.x, tile = 0, tile1 = 0, len = 0, block = 0, off = 0;
+  const int32_t* table = nullptr;
+  const char* head_codes = nullptr;
+  int64_t head_scales = 0, head_zeros = 0;
+  bool there = false;
+  auto look_up = [&]() -> bool {
+    while (tile == tile1 && k < n_items) {  // the first tile of the next item that has any
+      const Item it(p, k);
+      tile = it.e.tile0, tile1 = it.e.tile1, len = it.len;
+      table = a.block_table + it.e.seq * a.bt_stride;
+      head_codes = reinterpret_cast<const char*>(pl.codes) + it.head * pl.cs[2];
+      if constexpr (T::kQuant) {
+        head_scales = it.head * pl.ss[2];
+        head_zeros = it.head * pl.zs[2];
+      }
+      k += gridDim.x;
+    }
+    if (tile == tile1) return false;
+    const int t = tile * kTile + row;
+    there = t < len;
+    const int e = p.block_shift >= 0 ? t >> p.block_shift : t / a.block_size;
+    off = t - e * a.block_size;
+    block = there ? table[e] : 0;
+    ++tile;
+    return true;
+  };
+  bool pending = look_up();  // copies run ahead of the conversion, over the items' ends
+  auto copy = [&](char* dst) {  // the looked-up tile, if any
+    if (pending) {
+      const int64_t b = block < 0 ? 0 : block >= a.num_blocks ? a.num_blocks - 1 : block;
+      const char* src = there ? head_codes + b * pl.cs[0] + off * pl.cs[1] : nullptr;
+      const uint32_t lo = static_cast<uint32_t>(reinterpret_cast<uint64_t>(src));
+      const uint32_t hi = static_cast<uint32_t>(reinterpret_cast<uint64_t>(src) >> 32);
+      constexpr int n = T::kChunks, at_once = 32 / n;
+      const int chunk = lane % n;
+#pragma unroll
+      for (int i = 0; i < 32; i += at_once) {
+        const int r = i + lane / n;
+        const uint64_t from = static_cast<uint64_t>(__shfl_sync(~0u, hi, r)) << 32 | __shfl_sync(~0u, lo, r);
+        const int rr = w * 32 + r;
+        const uint32_t to = smem_addr(dst) + (T::kQuant ? T::at(rr, chunk)
+                                                        : (chunk >> 3) * (kTile * 128) + rr * 128 + (((chunk & 7) ^ (rr & 7)) << 4));
+        copy_async<16>(to, from ? reinterpret_cast<const char*>(from) + chunk * 16 : head_codes, from != 0);
+      }
+      if constexpr (T::kQuant) {
+        const int64_t so = there ? head_scales + b * pl.ss[0] + off * pl.ss[1] : 0;
+        copy_async<T::kScaleBytes>(smem_addr(dst + T::kScaleAt + row * T::kScaleBytes), pl.scales + so, there);
+        if constexpr (T::kBytes > T::kZeroAt) {
+          const int64_t zo = there ? head_zeros + b * pl.zs[0] + off * pl.zs[1] : 0;
+          copy_async<T::kScaleBytes>(smem_addr(dst + T::kZeroAt + row * T::kScaleBytes), pl.zeros + zo, there);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if constexpr (kStages > 0) {
+    for (int i = 0; i < kStages; ++i) {
+      copy(stages + i * T::kBytes);
+      pending = pending && look_up();
+    }
+  }
+  uint32_t done = SIDE, stage = 0;  // done: number of the plane tile in the ring's order
+  // The slot's use before this one, always the other plane's, has to be over.
+  auto wait_empty = [&]() {
+    const uint32_t others = (done / kRing + 1) / 2;  // uses of this slot by the other plane
+    mbar_wait(&mi.ring_empty[1 - SIDE][done % kRing], (others + 1) & 1, &mi.abort, p.status);
+  };
+  int serial = 0;
+  for (int ki = blockIdx.x; ki < n_items; ki += gridDim.x) {
+    const Item it(p, ki);
+    if (it.tiles() == 0) continue;
+    if constexpr (SIDE == 1 && T::kQuant) {
+      if (row == 0) {
+        mi.bad_count[serial % kBadLists] = 0;
+        mi.bad[serial % kBadLists][kBadMost] = make_int2(0x7fffffff, 0);
+      }
+      asm volatile("bar.sync 3, 128;" ::: "memory");
+    }
+    for (int j = 0; j < it.tiles(); ++j, done += 2) {
+      char* const to = sm + L::kRingAt + done % kRing * L::kTileBytes;
+        if constexpr (kStages == 0) {
+        wait_empty();
+        copy(to);
+        pending = pending && look_up();
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+      } else {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+        __syncwarp();
+        char* const from = stages + stage * T::kBytes;
+        if constexpr (SIDE == 1) {
+          // A value that is not finite would reach rows that do not attend to its token (as
+          // 0 x NaN): such groups are zeroed here and noted, and the rows that do attend to
+          // the token are made NaN at the end.
+          if (any_not_finite<MODE, D>(from, row)) {
+            const int bad = not_finite<MODE, D>(from, row);
+            for (int g = 0; g < D / 32; ++g) {
+              if (!(bad >> g & 1)) continue;
+              *reinterpret_cast<uint16_t*>(from + T::kScaleAt + row * T::kScaleBytes + 2 * g) = 0;
+              if constexpr (T::kBytes > T::kZeroAt)
+                *reinterpret_cast<uint16_t*>(from + T::kZeroAt + row * T::kScaleBytes + 2 * g) = 0;
+            }
+            const int token = (it.e.tile0 + j) * kTile + row;
+            const int at = atomicAdd(&mi.bad_count[serial % kBadLists], 1);
+            int2* list = mi.bad[serial % kBadLists];
+            if (at < kBadMost) {
+              list[at] = make_int2(token, bad);
+            } else {  // more than the list holds: from the first of them on, all their groups
+              atomicMin(&list[kBadMost].x, token);
+              atomicOr(&list[kBadMost].y, bad);
+            }
+          }
+        }
+        wait_empty();
+        dequantize_row<MODE, D>(from, to, row);
+      }
+      fence_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&mi.ring_full[done % kRing]);
+      if constexpr (kStages > 0) {
+        copy(stages + stage * T::kBytes);
+        pending = pending && look_up();
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+      }
+    }
+    ++serial;
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
 template <int KM, int VM, int D>
 __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_constant__ Params p) {
   using L = Layout<KM, VM, D>;
-  using KT = PlaneTile<KM, D>;
-  using VT = PlaneTile<VM, D>;
   extern __shared__ char smem_raw[];
   char* sm = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
   Misc& mi = *reinterpret_cast<Misc*>(sm + L::kMisc);
@@ -358,7 +552,7 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
   const ExtendArgs& a = p.a;
 
   if (tid == 0) {
-    for (int i = 0; i < kRing; ++i) mbar_init(&mi.ring_full[i], 4), mbar_init(&mi.ring_empty[i], 1);
+    for (int i = 0; i < kRing; ++i) mbar_init(&mi.ring_full[i], 4), mbar_init(&mi.ring_empty[0][i], 1), mbar_init(&mi.ring_empty[1][i], 1);
     mbar_init(&mi.q_full, 8);
     for (int w = 0; w < 2; ++w) {
       mbar_init(&mi.s_full[w], 1);
@@ -369,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (tid < kBadLists) mi.bad_count[tid] = 0;
-  if (warp == 12) {
+  if (warp == 16) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&mi.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -385,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
 
   if (warp < 8) {
     // ---------------------------------------------------------------- softmax streams
-    KNLP_REGISTERS("inc", 192);
+    KNLP_REGISTERS("inc", 136);
     const int w = warp >> 2, row = tid & 127;  // row: of the stream's 128
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // the warp's 32 TMEM lanes
     const uint32_t t_s = tmem + lanes + w * kTile, t_o = tmem + lanes + 256 + w * D;
@@ -445,19 +639,29 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
         wait(&mi.s_full[w], n_s++);
         fence_after();
         if (active) {
-          float s[kTile];
+          // Two halves of 64 columns; the first is read again after the maximum is known, which
+          // costs less than the registers that would hold all of S.
+          float s[64];
+          auto load = [&](int half) {
+            tmem_ld32(t_s + half * 64, reinterpret_cast<uint32_t*>(s));
+            tmem_ld32(t_s + half * 64 + 32, reinterpret_cast<uint32_t*>(s + 32));
+            tmem_wait_ld();
+            const int seen = limit - base - half * 64;
+            if (__any_sync(~0u, seen < 64)) {
 #pragma unroll
-          for (int i = 0; i < kTile; i += 32) tmem_ld32(t_s + i, reinterpret_cast<uint32_t*>(s + i));
-          tmem_wait_ld();
-          const int seen = limit - base;
-          if (__any_sync(~0u, seen < kTile)) {
+              for (int i = 0; i < 64; ++i) s[i] = i < seen ? s[i] : -INFINITY;
+            }
+          };
+          float mx[2] = {-INFINITY, -INFINITY};
+          auto maxima = [&]() {
 #pragma unroll
-            for (int i = 0; i < kTile; ++i) s[i] = i < seen ? s[i] : -INFINITY;
-          }
-          float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-          for (int i = 4; i < kTile; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
-          const float m_new = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c);
+            for (int i = 0; i < 64; i += 4) mx[0] = max3(mx[0], s[i], s[i + 1]), mx[1] = max3(mx[1], s[i + 2], s[i + 3]);
+          };
+          load(0);
+          maxima();
+          load(1);
+          maxima();
+          const float m_new = fmaxf(m, fmaxf(mx[0], mx[1]) * c);
           if (j == 0) {
             m = m_new;
           } else if (__any_sync(~0u, m_new > m + kGrow)) {
@@ -474,24 +678,29 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
               tmem_st32(t_o + i, o);
             }
           }
-          const float off = m == -INFINITY ? 0.0f : m;
-          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          const float off = m == -INFINITY ? 0.0f : -m;
+          const uint64_t c2 = pack2(c, c), off2 = pack2(off, off);
+          uint64_t sum[2] = {0, 0};
+          auto weights = [&](int half) {
             uint32_t pk[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-              const float x0 = fmaf(s[h * 64 + 2 * i], c, -off), x1 = fmaf(s[h * 64 + 2 * i + 1], c, -off);
-              float p0, p1;
+              float x0, x1, p0, p1;
+              unpack2(fma2(pack2(s[2 * i], s[2 * i + 1]), c2, off2), x0, x1);
               asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p0) : "f"(x0));
               asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p1) : "f"(x1));
-              sum[(2 * i) & 3] += p0;
-              sum[(2 * i + 1) & 3] += p1;
+              sum[i & 1] = add2(sum[i & 1], pack2(p0, p1));
               pk[i] = as_u32(__floats2half2_rn(p0, p1));
             }
-            tmem_st32(t_s + h * 32, pk);
-          }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tmem_st32(t_s + 64 + half * 32, pk);
+          };
+          // P overlays the second half of S, which is in registers by now
+          weights(1);
+          load(0);
+          weights(0);
+          float l0, l1;
+          unpack2(add2(sum[0], sum[1]), l0, l1);
+          l += l0 + l1;
           tmem_wait_st();
         }
         fence_before();
@@ -607,148 +816,45 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
       fence_before();
       serial += it.tiles() > 0;
     }
-  } else if (warp < 12) {
-    // ---------------------------------------------------------------- staging, dequantization
-    // Plane tiles in the order K0 V0 K1 V1 ..., item after item.  A warp stages and converts rows
-    // 32 w .. 32 w + 31 of every tile, a lane converts one row; only lanes of the same warp
-    // read what a lane has copied.
-    KNLP_REGISTERS("dec", 88);
-    const int w = warp - 8, row = w * 32 + lane;
-    struct Cursor {  // next plane tile to copy
-      int k, tile, tile1, len, head;
-      const int32_t* table;
-      int block, off;
-    } cur;
-    auto open = [&](Cursor& x, int k) {  // first tile of item k or of the first later one that has any
-      for (; k < n_items; k += gridDim.x) {
-        const Item it(p, k);
-        if (it.tiles() == 0) continue;
-        x.tile = it.e.tile0, x.tile1 = it.e.tile1, x.len = it.len, x.head = it.head;
-        x.table = a.block_table + it.e.seq * a.bt_stride;
-        break;
-      }
-      x.k = k;
-    };
-    open(cur, blockIdx.x);
-    uint32_t copied = 0;
-    auto copy_plane = [&](const Plane& pl, auto tag, char* stage, bool there) {
-      using T = decltype(tag);
-      const char* row_base = reinterpret_cast<const char*>(pl.codes) + cur.head * pl.cs[2];
-      constexpr int n = T::kChunks, rows_at_once = 32 / n;
-      const int chunk = lane % n;
-#pragma unroll
-      for (int i = 0; i < 32; i += rows_at_once) {
-        const int r = i + lane / n;
-        const int block = __shfl_sync(~0u, cur.block, r), off = __shfl_sync(~0u, cur.off, r);
-        const char* src = row_base + block * pl.cs[0] + off * pl.cs[1] + chunk * 16;
-        const bool ok = __shfl_sync(~0u, there, r);
-        copy_async<16>(smem_addr(stage + T::at(w * 32 + r, chunk)), ok ? src : row_base, ok);
-      }
-      if constexpr (T::kQuant) {
-        const int64_t so = cur.block * pl.ss[0] + cur.off * pl.ss[1] + cur.head * pl.ss[2];
-        copy_async<T::kScaleBytes>(smem_addr(stage + T::kScaleAt + row * T::kScaleBytes), pl.scales + (there ? so : 0), there);
-        if constexpr (T::kBytes > T::kZeroAt) {
-          const int64_t zo = cur.block * pl.zs[0] + cur.off * pl.zs[1] + cur.head * pl.zs[2];
-          copy_async<T::kScaleBytes>(smem_addr(stage + T::kZeroAt + row * T::kScaleBytes), pl.zeros + (there ? zo : 0), there);
-        }
-      }
-    };
-    auto copy_next = [&]() {
-      if (cur.k < n_items) {
-        char* stage = sm + L::kStageAt + copied % L::kStages * L::kStageBytes;
-        const int t = cur.tile * kTile + row;
-        const bool there = t < cur.len;
-        if (copied & 1) {
-          copy_plane(a.v, VT{}, stage, there);
-          if (++cur.tile == cur.tile1) open(cur, cur.k + gridDim.x);
-        } else {
-          const int e = t / a.block_size;
-          int64_t block = there ? cur.table[e] : 0;
-          block = block < 0 ? 0 : block >= a.num_blocks ? a.num_blocks - 1 : block;
-          cur.block = static_cast<int>(block);
-          cur.off = t - e * a.block_size;
-          copy_plane(a.k, KT{}, stage, there);
-        }
-        ++copied;
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    for (int i = 0; i < L::kStages - 1; ++i) copy_next();
-    uint32_t done = 0;
-    int serial = 0;
-    for (int k = blockIdx.x; k < n_items; k += gridDim.x) {
-      const Item it(p, k);
-      if (it.tiles() == 0) continue;
-      if (row == 0) {
-        mi.bad_count[serial % kBadLists] = 0;
-        mi.bad[serial % kBadLists][kBadMost] = make_int2(0x7fffffff, 0);
-      }
-      asm volatile("bar.sync 3, 128;" ::: "memory");
-      for (int j = 0; j < it.tiles(); ++j) {
-#pragma unroll
-        for (int plane = 0; plane < 2; ++plane, ++done) {
-          asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 2) : "memory");
-          __syncwarp();
-          char* stage = sm + L::kStageAt + done % L::kStages * L::kStageBytes;
-          char* tile = sm + L::kRingAt + done % kRing * L::kTileBytes;
-          wait(&mi.ring_empty[done % kRing], done / kRing + 1);
-          if (plane == 0) {
-            dequantize_row<KM, D>(stage, tile, row);
-          } else {
-            // A value that is not finite would reach rows that do not attend to its token (as
-            // 0 x NaN): such groups are zeroed here and noted, and the rows that do attend
-            // to the token are made NaN at the end.
-            const int bad = not_finite<VM, D>(stage, row);
-            if (bad) {
-              char* sc = stage + VT::kScaleAt + row * VT::kScaleBytes;
-              for (int g = 0; g < D / 32; ++g) {
-                if (!(bad >> g & 1)) continue;
-                *reinterpret_cast<uint16_t*>(sc + 2 * g) = 0;
-                if constexpr (VT::kBytes > VT::kZeroAt)
-                  *reinterpret_cast<uint16_t*>(stage + VT::kZeroAt + row * VT::kScaleBytes + 2 * g) = 0;
-              }
-              const int token = (it.e.tile0 + j) * kTile + row;
-              const int at = atomicAdd(&mi.bad_count[serial % kBadLists], 1);
-              int2* list = mi.bad[serial % kBadLists];
-              if (at < kBadMost) {
-                list[at] = make_int2(token, bad);
-              } else {  // more than the list holds: from the first of them on, all their groups
-                atomicMin(&list[kBadMost].x, token);
-                atomicOr(&list[kBadMost].y, bad);
-              }
-            }
-            dequantize_row<VM, D>(stage, tile, row);
-          }
-          fence_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&mi.ring_full[done % kRing]);
-          copy_next();
-        }
-      }
-      ++serial;
-    }
-    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp < 16) {
+    KNLP_REGISTERS("dec", 80);
+    if (warp < 12) produce<L, KM, D, 0>(p, sm, mi, n_items, warp - 8, lane);
+    else produce<L, VM, D, 1>(p, sm, mi, n_items, warp - 12, lane);
   } else {
     // ---------------------------------------------------------------- matrix products
-    KNLP_REGISTERS("dec", 40);
-    if (warp == 12 && lane == 0) {
-      const uint32_t q_at = smem_addr(sm + L::kQ), ring_at = smem_addr(sm + L::kRingAt);
+    KNLP_REGISTERS("dec", 48);
+    if (warp == 16) {
+      // The whole warp follows the items and waits; one lane issues.
+      const uint64_t q_at = operand(smem_addr(sm + L::kQ), 16, 1024);
+      const uint64_t k_at = operand(smem_addr(sm + L::kRingAt), 16, 1024);
+      const uint64_t v_at = operand(smem_addr(sm + L::kRingAt), kTile * 128, 1024);
       const uint32_t idesc_s = product(kRows, kTile, raw_bf16, false);
       const uint32_t idesc_o = product(kRows, D, false, true);
-      uint32_t used = 0, n_q = 0, n_p[2] = {0, 0};
-      auto scores = [&](int w, int qt, uint32_t slot) {  // S of stream w = Q tile qt x K tile
-        const uint32_t q = q_at + qt * L::kTileBytes, kk = ring_at + slot * L::kTileBytes;
+      uint32_t used = 0, n_q = 0, p_phase = 0;  // p_phase: bit w for stream w
+      // S of stream w = Q tile qt x K tile, then the barriers that its end completes
+      auto scores = [&](int w, int qt, uint32_t slot, bool last_use) {
+        const uint64_t q = q_at + (qt * L::kTileBytes >> 4), kk = k_at + (slot * L::kTileBytes >> 4);
+        if (elect()) {
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          const uint32_t off = (i >> 2) * (kTile * 128) + (i & 3) * 32;
-          mma_ss(tmem + w * kTile, operand(q + off, 16, 1024), operand(kk + off, 16, 1024), idesc_s, i > 0);
+          for (int i = 0; i < D / 16; ++i) {
+            const int off = ((i >> 2) * (kTile * 128) + (i & 3) * 32) >> 4;
+            mma_ss(tmem + w * kTile, q + off, kk + off, idesc_s, i > 0);
+          }
+          commit(&mi.s_full[w]);
+          if (last_use) commit(&mi.ring_empty[0][slot]);
         }
+        __syncwarp();
       };
-      auto values = [&](int w, uint32_t slot, bool acc) {  // O of stream w += P x V tile
-        const uint32_t v = ring_at + slot * L::kTileBytes;
+      auto values = [&](int w, uint32_t slot, bool acc, bool last_use, bool last) {  // O of stream w += P x V tile
+        const uint64_t v = v_at + (slot * L::kTileBytes >> 4);
+        if (elect()) {
 #pragma unroll
-        for (int i = 0; i < kTile / 16; ++i)
-          mma_ts(tmem + 256 + w * D, tmem + w * kTile + i * 8, operand(v + i * 2048, kTile * 128, 1024), idesc_o, acc || i > 0);
+          for (int i = 0; i < kTile / 16; ++i)
+            mma_ts(tmem + 256 + w * D, tmem + w * kTile + 64 + i * 8, v + (i * 2048 >> 4), idesc_o, acc || i > 0);
+          if (last_use) commit(&mi.ring_empty[1][slot]);
+          if (last) commit(&mi.o_full[w]);
+        }
+        __syncwarp();
       };
       auto ready = [&](uint32_t x) {  // plane tile x of the ring
         wait(&mi.ring_full[x % kRing], x / kRing);
@@ -756,7 +862,8 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
         return x % kRing;
       };
       auto probs = [&](int w) {
-        wait(&mi.p_full[w], n_p[w]++);
+        wait(&mi.p_full[w], p_phase >> w);
+        p_phase ^= 1u << w;
         fence_after();
       };
       for (int k = blockIdx.x; k < n_items; k += gridDim.x) {
@@ -767,47 +874,29 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
         fence_after();
         if (it.pair()) {
           uint32_t slot = ready(used);
-          scores(0, 0, slot), commit(&mi.s_full[0]);
-          scores(1, 1, slot), commit(&mi.s_full[1]);
-          commit(&mi.ring_empty[slot]);
+          scores(0, 0, slot, false);
+          scores(1, 1, slot, true);
           for (int j = 0; j < n; ++j, used += 2) {
             const bool more = j + 1 < n;
             const uint32_t v = ready(used + 1);
             probs(0);
-            values(0, v, j > 0);
+            values(0, v, j > 0, false, !more);
             if (more) {
               slot = ready(used + 2);
-              scores(0, 0, slot), commit(&mi.s_full[0]);
-            } else {
-              commit(&mi.o_full[0]);
+              scores(0, 0, slot, false);
             }
             probs(1);
-            values(1, v, j > 0);
-            commit(&mi.ring_empty[v]);
-            if (more) {
-              scores(1, 1, slot), commit(&mi.s_full[1]);
-              commit(&mi.ring_empty[slot]);
-            } else {
-              commit(&mi.o_full[1]);
-            }
+            values(1, v, j > 0, true, !more);
+            if (more) scores(1, 1, slot, true);
           }
         } else {
-          for (int w = 0; w < 2 && w < n; ++w) {
-            const uint32_t slot = ready(used + 2 * w);
-            scores(w, 0, slot), commit(&mi.s_full[w]), commit(&mi.ring_empty[slot]);
-          }
+          for (int w = 0; w < 2 && w < n; ++w) scores(w, 0, ready(used + 2 * w), true);
           for (int j = 0; j < n; ++j, used += 2) {
             const int w = j & 1;
             const uint32_t v = ready(used + 1);
             probs(w);
-            values(w, v, j > 1);
-            commit(&mi.ring_empty[v]);
-            if (j + 2 < n) {
-              const uint32_t slot = ready(used + 4);
-              scores(w, 0, slot), commit(&mi.s_full[w]), commit(&mi.ring_empty[slot]);
-            } else {
-              commit(&mi.o_full[w]);
-            }
+            values(w, v, j > 1, true, j + 2 >= n);
+            if (j + 2 < n) scores(w, 0, ready(used + 4), true);
           }
         }
       }
@@ -818,7 +907,7 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
   fence_before();
   __syncthreads();
   fence_after();
-  if (warp == 12)
+  if (warp == 16)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 

@@ -335,6 +335,9 @@ int launch_extend_mma(const ExtendArgs& a, float* ws, int64_t ws_floats, int n_s
   p.status = decode_status_ptr();
   if (!p.status) return KNLP_ERR_NO_DEVICE;
   p.rep = a.n_q_heads / a.n_kv_heads;
+  p.block_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (a.block_size == 1 << i) p.block_shift = i;
   extend_plan_kernel<<<1, kPlanThreads, 0, st>>>(a, p.rep, n_sms, static_cast<int>(z.entries),
                                                  static_cast<int>(z.splits), z.parts, base, plan,
                                                  entries, splits);

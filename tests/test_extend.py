@@ -164,6 +164,8 @@ class Batch:
         assert torch.equal(l[:T].isfinite(), fin) and (l[:T][~fin] == -math.inf).all()
         assert ((l[:T].double() - lse[:T]).abs()[fin] <= bl[:T][fin]).all()
         assert (r[:T][~fin] == 0).all()
+        from knlp_b200 import ops
+        assert ops.device_status() == 0  # no wait inside a kernel ran out
         return r
 
 
