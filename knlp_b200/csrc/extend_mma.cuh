@@ -10,7 +10,7 @@
 // cycle), below that HBM.  Work items and their split over CTAs: extend_plan.cu.
 //
 // One CTA per SM (it owns all 512 TMEM columns), 20 warps whose registers are dealt out by
-// setmaxnreg (2 x 136 + 2 x 80 + 48 = 5 x 96 a lane):
+// setmaxnreg (2 x 144 + 2 x 72 + 48 = 5 x 96 a lane):
 //   warps 0-3, 4-7   two softmax streams, a thread per query row.  An item of more than 128 rows
 //                    gives each stream its own 128 rows over the same K / V tiles; a smaller
 //                    one gives both streams the same rows and every other tile, and their
@@ -122,10 +122,15 @@ struct Layout {
   static_assert(kBytes <= 232448, "shared memory of an SM");
 };
 
+template <int N>
+struct Int {
+  static constexpr int value = N;
+};
+
 struct Misc {
   uint64_t ring_full[kRing];
   uint64_t ring_empty[2][kRing];  // a K tile, a V tile in the slot has been used
-  uint64_t q_full, s_full[2], p_full[2], o_full[2];
+  uint64_t q_full, s_full[2], p_half[2], p_full[2], o_full[2];
   uint32_t tmem;
   int abort;
   float m[kRows], l[kRows];  // second stream's state when both serve the same rows
@@ -203,32 +208,49 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
         "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// The wait names the registers of the load, so that no use of them moves above it.
+__device__ __forceinline__ void tmem_wait_ld(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+      : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+        "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+        "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+        "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+      :: "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Shared-memory operand descriptor, 128-byte swizzle.  K-major operands (Q, K): rows of 128
-// bytes in groups of eight, `stride` between groups.  MN-major operand (V as stored, a row per
-// token): `lead` between blocks of 64 columns, `stride` between groups of eight tokens.
-__device__ __forceinline__ uint64_t operand(uint32_t addr, int lead, int stride) {
-  return static_cast<uint64_t>((addr >> 4) & 0x3fff) | static_cast<uint64_t>(lead >> 4) << 16 |
-         static_cast<uint64_t>(stride >> 4) << 32 | 1ull << 46 | 2ull << 61;
+// Shared-memory operand descriptor, 128-byte swizzle, groups of eight 128-byte rows 1024 bytes
+// apart.  K-major operands (Q, K): a row per query row / token.  MN-major operand (V as stored, a
+// row per token): `lead` bytes between blocks of 64 columns.  Only the low word varies.
+constexpr uint32_t kOperandHigh = 1024 >> 4 | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t operand(uint32_t addr, int lead) {
+  return addr >> 4 | static_cast<uint32_t>(lead >> 4) << 16;
 }
 // Instruction descriptor: fp32 accumulator, fp16 or bf16 inputs, B optionally MN-major.
 __host__ __device__ constexpr uint32_t product(int m, int n, bool bf16, bool b_mn) {
   return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (b_mn ? 1u << 16 : 0u) |
          static_cast<uint32_t>(n >> 3) << 17 | static_cast<uint32_t>(m >> 4) << 24;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+// D (+)= A B, both operands in shared memory at OFF 16-byte units behind a and b.  The
+// descriptors are put together here: kept outside they would not fit the warp's registers.
+template <int OFF>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
   asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc)) : "memory");
+      "{\n.reg .pred p;\n.reg .b32 x, y;\n.reg .b64 da, db;\n"
+      "add.u32 x, %1, %5;\nadd.u32 y, %2, %5;\n"
+      "mov.b64 da, {x, %6};\nmov.b64 db, {y, %6};\nsetp.ne.u32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}"
+      ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc)), "n"(OFF), "n"(kOperandHigh) : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+// The same with A in TMEM, at COL columns behind a.
+template <int COL, int OFF>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
   asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
-      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc)) : "memory");
+      "{\n.reg .pred p;\n.reg .b32 x, y;\n.reg .b64 db;\n"
+      "add.u32 x, %1, %7;\nadd.u32 y, %2, %5;\n"
+      "mov.b64 db, {y, %6};\nsetp.ne.u32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [x], db, %3, p;\n}"
+      ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(static_cast<uint32_t>(acc)), "n"(OFF), "n"(kOperandHigh), "n"(COL) : "memory");
 }
 
 // One lane of the converged warp.
@@ -250,6 +272,30 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool t
 
 __device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+      : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+        "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+      :: "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 
 // Two fp32 lanes in one instruction, and the maximum of three.
 __device__ __forceinline__ uint64_t pack2(float x, float y) {
@@ -556,6 +602,7 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
     mbar_init(&mi.q_full, 8);
     for (int w = 0; w < 2; ++w) {
       mbar_init(&mi.s_full[w], 1);
+      mbar_init(&mi.p_half[w], 4);
       mbar_init(&mi.p_full[w], 4);
       mbar_init(&mi.o_full[w], 1);
     }
@@ -579,22 +626,37 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
 
   if (warp < 8) {
     // ---------------------------------------------------------------- softmax streams
-    KNLP_REGISTERS("inc", 136);
+    KNLP_REGISTERS("inc", 144);
     const int w = warp >> 2, row = tid & 127;  // row: of the stream's 128
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // the warp's 32 TMEM lanes
     const uint32_t t_s = tmem + lanes + w * kTile, t_o = tmem + lanes + 256 + w * D;
     const float c = a.scale * kLog2e;
     uint32_t n_s = 0, n_o = 0;
     int serial = 0;
+    // A thread's row of an item, derived anew behind the tiles: it would not fit the registers
+    // beside S.
+    struct Row {
+      int local, flat, tok, limit;
+      bool valid, active;  // of the thread; of its warp
+      __device__ Row(const Params& p, const Item& it, int w, int row) {
+        const int first = it.pair() ? w * kRows : 0;
+        local = first + row;
+        valid = local < it.e.rows;
+        active = first + (row & ~31) < it.e.rows;
+        flat = it.e.row0 + local;
+        tok = flat / p.rep;
+        limit = !valid ? 0 : p.a.causal ? max(min(it.ctx + tok + 1, it.len), 0) : it.len;
+      }
+    };
     for (int k = blockIdx.x; k < n_items; k += gridDim.x) {
+      float m = -INFINITY, l = 0.0f;
+      {
       const Item it(p, k);
       const int tiles = it.tiles_of(w);
-      const int local = (it.pair() ? w * kRows : 0) + row;  // row of the item
-      const bool valid = local < it.e.rows;
-      const int flat = it.e.row0 + local;
-      const int tok = flat / p.rep;
-      const int limit = !valid ? 0 : a.causal ? max(min(it.ctx + tok + 1, it.len), 0) : it.len;
-      const bool active = (it.pair() ? w * kRows : 0) + (row & ~31) < it.e.rows;  // of the warp
+      const Row rw(p, it, w, row);
+      const int limit = rw.limit;
+      const bool active = rw.active;
+      const int whole = __reduce_min_sync(~0u, rw.valid ? limit : 0x7fffffff);  // of the warp's rows
 
       asm volatile("bar.sync 1, 256;" ::: "memory");  // nobody reads the Q area any more
       if (it.tiles() && (w == 0 || it.pair())) {
@@ -633,34 +695,38 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
       __syncwarp();
       if (it.tiles() && lane == 0) mbar_arrive(&mi.q_full);
 
-      float m = -INFINITY, l = 0.0f;
-      for (int j = 0; j < tiles; ++j) {
-        const int base = (it.e.tile0 + (it.pair() ? j : 2 * j + w)) * kTile;
+      const int step = it.pair() ? kTile : 2 * kTile;
+      int base = (it.e.tile0 + (it.pair() ? 0 : w)) * kTile;
+      for (int j = 0; j < tiles; ++j, base += step) {
         wait(&mi.s_full[w], n_s++);
         fence_after();
-        if (active) {
-          // Two halves of 64 columns; the first is read again after the maximum is known, which
+        // cut: some row of the warp ends inside the tile
+        auto tile = [&](auto cut) {
+          // Four chunks of 32 columns in two register buffers, each load under the work on the
+          // chunk before.  The first two chunks are read again once the maximum is known, which
           // costs less than the registers that would hold all of S.
-          float s[64];
-          auto load = [&](int half) {
-            tmem_ld32(t_s + half * 64, reinterpret_cast<uint32_t*>(s));
-            tmem_ld32(t_s + half * 64 + 32, reinterpret_cast<uint32_t*>(s + 32));
-            tmem_wait_ld();
-            const int seen = limit - base - half * 64;
-            if (__any_sync(~0u, seen < 64)) {
+          float x0[32], x1[32];
+          auto ask = [&](int chunk, float* x) { tmem_ld32(t_s + chunk * 32, reinterpret_cast<uint32_t*>(x)); };
+          auto got = [&](int chunk, float* x) {
+            tmem_wait_ld(reinterpret_cast<uint32_t*>(x));
+            if constexpr (decltype(cut)::value) {
+              const int seen = limit - base - chunk * 32;
+              uint32_t mask = seen >= 32 ? ~0u : seen <= 0 ? 0u : (1u << seen) - 1;
+              asm volatile("" : "+r"(mask));  // one register, not 32 predicates kept for later
 #pragma unroll
-              for (int i = 0; i < 64; ++i) s[i] = i < seen ? s[i] : -INFINITY;
+              for (int i = 0; i < 32; ++i) x[i] = mask >> i & 1 ? x[i] : -INFINITY;
             }
           };
           float mx[2] = {-INFINITY, -INFINITY};
-          auto maxima = [&]() {
+          auto maxima = [&](const float* x) {
 #pragma unroll
-            for (int i = 0; i < 64; i += 4) mx[0] = max3(mx[0], s[i], s[i + 1]), mx[1] = max3(mx[1], s[i + 2], s[i + 3]);
+            for (int i = 0; i < 32; i += 4) mx[0] = max3(mx[0], x[i], x[i + 1]), mx[1] = max3(mx[1], x[i + 2], x[i + 3]);
           };
-          load(0);
-          maxima();
-          load(1);
-          maxima();
+          ask(0, x0), got(0, x0);
+          ask(1, x1), maxima(x0), got(1, x1);
+          ask(2, x0), maxima(x1), got(2, x0);
+          ask(3, x1), maxima(x0), got(3, x1);
+          maxima(x1);
           const float m_new = fmaxf(m, fmaxf(mx[0], mx[1]) * c);
           if (j == 0) {
             m = m_new;
@@ -668,47 +734,66 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
             const float f = m_new == m ? 1.0f : exp2f(m - m_new);
             m = m_new;
             l *= f;
+#pragma unroll 1
+            for (int i = 0; i < D; i += 16) {
+              uint32_t o[16];
+              tmem_ld16(t_o + i, o);
+              tmem_wait_ld16(o);
 #pragma unroll
-            for (int i = 0; i < D; i += 32) {
-              uint32_t o[32];
-              tmem_ld32(t_o + i, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-              tmem_st32(t_o + i, o);
+              for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+              tmem_st16(t_o + i, o);
             }
           }
           const float off = m == -INFINITY ? 0.0f : -m;
           const uint64_t c2 = pack2(c, c), off2 = pack2(off, off);
           uint64_t sum[2] = {0, 0};
-          auto weights = [&](int half) {
-            uint32_t pk[32];
+          // P overlays the second half of S, whose chunks are in registers by now
+          auto weights = [&](int chunk, const float* x) {
+            uint32_t pk[16];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              float x0, x1, p0, p1;
-              unpack2(fma2(pack2(s[2 * i], s[2 * i + 1]), c2, off2), x0, x1);
-              asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p0) : "f"(x0));
-              asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p1) : "f"(x1));
+            for (int i = 0; i < 16; ++i) {
+              float y0, y1, p0, p1;
+              unpack2(fma2(pack2(x[2 * i], x[2 * i + 1]), c2, off2), y0, y1);
+              asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p0) : "f"(y0));
+              asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p1) : "f"(y1));
               sum[i & 1] = add2(sum[i & 1], pack2(p0, p1));
               pk[i] = as_u32(__floats2half2_rn(p0, p1));
             }
-            tmem_st32(t_s + 64 + half * 32, pk);
+            tmem_st16(t_s + 64 + chunk * 16, pk);
           };
-          // P overlays the second half of S, which is in registers by now
-          weights(1);
-          load(0);
-          weights(0);
+          weights(2, x0);
+          ask(0, x0);
+          weights(3, x1);
+          tmem_wait_st();
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&mi.p_half[w]);  // the products with the second half may start
+          got(0, x0);
+          ask(1, x1);
+          weights(0, x0);
+          got(1, x1);
+          weights(1, x1);
           float l0, l1;
           unpack2(add2(sum[0], sum[1]), l0, l1);
           l += l0 + l1;
           tmem_wait_st();
+        };
+        if (active) {
+          if (base + kTile > whole) tile(Int<1>{});
+          else tile(Int<0>{});
+        } else if (lane == 0) {
+          mbar_arrive(&mi.p_half[w]);
         }
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&mi.p_full[w]);
       }
 
+      }
       // ---- epilogue
+      const Item it(p, k);
+      const int tiles = it.tiles_of(w);
+      const auto [local, flat, tok, limit, valid, active] = Row(p, it, w, row);
       if (tiles) {
         wait(&mi.o_full[w], n_o++);
         fence_after();
@@ -721,7 +806,7 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
           for (int i = 0; i < D; i += 32) {
             uint32_t o[32];
             tmem_ld32(t_o + i, o);
-            tmem_wait_ld();
+            tmem_wait_ld(o);
 #pragma unroll
             for (int x = 0; x < 32; ++x) swap[(i + x) * kRows + row] = __uint_as_float(o[x]);
           }
@@ -752,7 +837,7 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
           float o[32];
           if (tiles) {
             tmem_ld32(t_o + i, reinterpret_cast<uint32_t*>(o));
-            tmem_wait_ld();
+            tmem_wait_ld(reinterpret_cast<uint32_t*>(o));
           } else {
 #pragma unroll
             for (int x = 0; x < 32; ++x) o[x] = 0.0f;
@@ -817,7 +902,7 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
       serial += it.tiles() > 0;
     }
   } else if (warp < 16) {
-    KNLP_REGISTERS("dec", 80);
+    KNLP_REGISTERS("dec", 72);
     if (warp < 12) produce<L, KM, D, 0>(p, sm, mi, n_items, warp - 8, lane);
     else produce<L, VM, D, 1>(p, sm, mi, n_items, warp - 12, lane);
   } else {
@@ -825,32 +910,45 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
     KNLP_REGISTERS("dec", 48);
     if (warp == 16) {
       // The whole warp follows the items and waits; one lane issues.
-      const uint64_t q_at = operand(smem_addr(sm + L::kQ), 16, 1024);
-      const uint64_t k_at = operand(smem_addr(sm + L::kRingAt), 16, 1024);
-      const uint64_t v_at = operand(smem_addr(sm + L::kRingAt), kTile * 128, 1024);
+      const uint32_t q_at = operand(smem_addr(sm + L::kQ), 16);
+      const uint32_t k_at = operand(smem_addr(sm + L::kRingAt), 16);
+      const uint32_t v_at = operand(smem_addr(sm + L::kRingAt), kTile * 128);
       const uint32_t idesc_s = product(kRows, kTile, raw_bf16, false);
-      const uint32_t idesc_o = product(kRows, D, false, true);
+      constexpr uint32_t idesc_o = product(kRows, D, false, true);
       uint32_t used = 0, n_q = 0, p_phase = 0;  // p_phase: bit w for stream w
       // S of stream w = Q tile qt x K tile, then the barriers that its end completes
       auto scores = [&](int w, int qt, uint32_t slot, bool last_use) {
-        const uint64_t q = q_at + (qt * L::kTileBytes >> 4), kk = k_at + (slot * L::kTileBytes >> 4);
+        const uint32_t q = q_at + (qt * L::kTileBytes >> 4), kk = k_at + (slot * L::kTileBytes >> 4);
+        const uint32_t d = tmem + w * kTile;
         if (elect()) {
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            const int off = ((i >> 2) * (kTile * 128) + (i & 3) * 32) >> 4;
-            mma_ss(tmem + w * kTile, q + off, kk + off, idesc_s, i > 0);
-          }
+          auto step = [&](auto i) {
+            constexpr int n = decltype(i)::value;
+            mma_ss<((n >> 2) * (kTile * 128) + (n & 3) * 32) / 16>(d, q, kk, idesc_s, n > 0);
+          };
+          step(Int<0>{}), step(Int<1>{}), step(Int<2>{}), step(Int<3>{});
+          if constexpr (D == 128) step(Int<4>{}), step(Int<5>{}), step(Int<6>{}), step(Int<7>{});
           commit(&mi.s_full[w]);
           if (last_use) commit(&mi.ring_empty[0][slot]);
         }
         __syncwarp();
       };
-      auto values = [&](int w, uint32_t slot, bool acc, bool last_use, bool last) {  // O of stream w += P x V tile
-        const uint64_t v = v_at + (slot * L::kTileBytes >> 4);
+      // O of stream w += P x V tile, second half of the tokens first, as P is written
+      auto values = [&](int w, uint32_t slot, bool acc, bool last_use, bool last) {
+        const uint32_t v = v_at + (slot * L::kTileBytes >> 4);
+        const uint32_t d = tmem + 256 + w * D, pr = tmem + w * kTile + 64;
+        auto step = [&](auto i, bool add) {
+          constexpr int n = decltype(i)::value;
+          mma_ts<n * 8, n * 2048 / 16>(d, pr, v, idesc_o, add);
+        };
+        wait(&mi.p_half[w], p_phase >> w);
+        fence_after();
+        if (elect()) step(Int<4>{}, acc), step(Int<5>{}, true), step(Int<6>{}, true), step(Int<7>{}, true);
+        __syncwarp();
+        wait(&mi.p_full[w], p_phase >> w);
+        p_phase ^= 1u << w;
+        fence_after();
         if (elect()) {
-#pragma unroll
-          for (int i = 0; i < kTile / 16; ++i)
-            mma_ts(tmem + 256 + w * D, tmem + w * kTile + 64 + i * 8, v + (i * 2048 >> 4), idesc_o, acc || i > 0);
+          step(Int<0>{}, true), step(Int<1>{}, true), step(Int<2>{}, true), step(Int<3>{}, true);
           if (last_use) commit(&mi.ring_empty[1][slot]);
           if (last) commit(&mi.o_full[w]);
         }
@@ -861,44 +959,23 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
         fence_after();
         return x % kRing;
       };
-      auto probs = [&](int w) {
-        wait(&mi.p_full[w], p_phase >> w);
-        p_phase ^= 1u << w;
-        fence_after();
-      };
       for (int k = blockIdx.x; k < n_items; k += gridDim.x) {
         const Item it(p, k);
         const int n = it.tiles();
         if (n == 0) continue;
         wait(&mi.q_full, n_q++);
         fence_after();
-        if (it.pair()) {
-          uint32_t slot = ready(used);
-          scores(0, 0, slot, false);
-          scores(1, 1, slot, true);
-          for (int j = 0; j < n; ++j, used += 2) {
-            const bool more = j + 1 < n;
-            const uint32_t v = ready(used + 1);
-            probs(0);
-            values(0, v, j > 0, false, !more);
-            if (more) {
-              slot = ready(used + 2);
-              scores(0, 0, slot, false);
-            }
-            probs(1);
-            values(1, v, j > 0, true, !more);
-            if (more) scores(1, 1, slot, true);
-          }
-        } else {
-          for (int w = 0; w < 2 && w < n; ++w) scores(w, 0, ready(used + 2 * w), true);
-          for (int j = 0; j < n; ++j, used += 2) {
-            const int w = j & 1;
-            const uint32_t v = ready(used + 1);
-            probs(w);
-            values(w, v, j > 1, true, j + 2 >= n);
-            if (j + 2 < n) scores(w, 0, ready(used + 4), true);
-          }
+        // Steps alternate between the streams: the output of one, then its next scores.  The
+        // first two steps have scores only.  Of a pair, both streams use every K / V tile.
+        const bool pair = it.pair();
+        const int steps = pair ? 2 * n : n;
+        for (int i = -2; i < steps; ++i) {
+          const int w = i & 1, j = pair ? i >> 1 : i, next = pair ? j + 1 : j + 2;
+          const bool last_use = !pair || w;
+          if (i >= 0) values(w, ready(used + 2 * j + 1), pair ? j > 0 : j > 1, last_use, next >= n);
+          if (next < n) scores(w, pair ? w : 0, ready(used + 2 * next), last_use);
         }
+        used += 2 * n;
       }
     }
     __syncwarp();
