@@ -10,7 +10,7 @@
 // cycle), below that HBM.  Work items and their split over CTAs: extend_plan.cu.
 //
 // One CTA per SM (it owns all 512 TMEM columns), 20 warps whose registers are dealt out by
-// setmaxnreg (2 x 144 + 2 x 72 + 48 = 5 x 96 a lane):
+// setmaxnreg (2 x 136 + 2 x 80 + 48 = 5 x 96 a lane):
 //   warps 0-3, 4-7   two softmax streams, a thread per query row.  An item of more than 128 rows
 //                    gives each stream its own 128 rows over the same K / V tiles; a smaller
 //                    one gives both streams the same rows and every other tile, and their
@@ -130,7 +130,7 @@ struct Int {
 struct Misc {
   uint64_t ring_full[kRing];
   uint64_t ring_empty[2][kRing];  // a K tile, a V tile in the slot has been used
-  uint64_t q_full, s_full[2], p_half[2], p_full[2], o_full[2];
+  uint64_t q_full, s_full[2], p_half[2], p_full[2], o_half[2], o_full[2];
   uint32_t tmem;
   int abort;
   float m[kRows], l[kRows];  // second stream's state when both serve the same rows
@@ -175,6 +175,16 @@ __device__ __forceinline__ void mbar_wait_long(uint64_t* b, uint32_t parity, vol
 }
 __device__ __forceinline__ void mbar_wait(uint64_t* b, uint32_t parity, int* abort, int* status) {
   if (!mbar_try(b, parity)) mbar_wait_long(b, parity, abort, status);
+}
+
+// A value that all lanes hold, in a uniform register: descriptors made from it need no moves.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __reduce_or_sync(~0u, x); }
+// The same wait for a converged warp, with a uniform branch.
+__device__ __forceinline__ void mbar_wait_warp(uint64_t* b, uint32_t parity, int* abort, int* status) {
+  if (!__all_sync(~0u, mbar_try(b, parity))) {
+    mbar_wait_long(b, parity, abort, status);
+    __syncwarp();
+  }
 }
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -604,6 +614,7 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
       mbar_init(&mi.s_full[w], 1);
       mbar_init(&mi.p_half[w], 4);
       mbar_init(&mi.p_full[w], 4);
+      mbar_init(&mi.o_half[w], 1);
       mbar_init(&mi.o_full[w], 1);
     }
     mi.abort = 0;
@@ -626,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
 
   if (warp < 8) {
     // ---------------------------------------------------------------- softmax streams
-    KNLP_REGISTERS("inc", 144);
+    KNLP_REGISTERS("inc", 136);
     const int w = warp >> 2, row = tid & 127;  // row: of the stream's 128
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // the warp's 32 TMEM lanes
     const uint32_t t_s = tmem + lanes + w * kTile, t_o = tmem + lanes + 256 + w * D;
@@ -700,93 +711,84 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
       for (int j = 0; j < tiles; ++j, base += step) {
         wait(&mi.s_full[w], n_s++);
         fence_after();
-        // cut: some row of the warp ends inside the tile
-        auto tile = [&](auto cut) {
-          // Four chunks of 32 columns in two register buffers, each load under the work on the
-          // chunk before.  The first two chunks are read again once the maximum is known, which
-          // costs less than the registers that would hold all of S.
-          float x0[32], x1[32];
-          auto ask = [&](int chunk, float* x) { tmem_ld32(t_s + chunk * 32, reinterpret_cast<uint32_t*>(x)); };
-          auto got = [&](int chunk, float* x) {
-            tmem_wait_ld(reinterpret_cast<uint32_t*>(x));
-            if constexpr (decltype(cut)::value) {
-              const int seen = limit - base - chunk * 32;
-              uint32_t mask = seen >= 32 ? ~0u : seen <= 0 ? 0u : (1u << seen) - 1;
-              asm volatile("" : "+r"(mask));  // one register, not 32 predicates kept for later
-#pragma unroll
-              for (int i = 0; i < 32; ++i) x[i] = mask >> i & 1 ? x[i] : -INFINITY;
-            }
-          };
-          float mx[2] = {-INFINITY, -INFINITY};
-          auto maxima = [&](const float* x) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) mx[0] = max3(mx[0], x[i], x[i + 1]), mx[1] = max3(mx[1], x[i + 2], x[i + 3]);
-          };
-          ask(0, x0), got(0, x0);
-          ask(1, x1), maxima(x0), got(1, x1);
-          ask(2, x0), maxima(x1), got(2, x0);
-          ask(3, x1), maxima(x0), got(3, x1);
-          maxima(x1);
-          const float m_new = fmaxf(m, fmaxf(mx[0], mx[1]) * c);
-          if (j == 0) {
-            m = m_new;
-          } else if (__any_sync(~0u, m_new > m + kGrow)) {
-            const float f = m_new == m ? 1.0f : exp2f(m - m_new);
-            m = m_new;
-            l *= f;
+        // Two halves of 64 tokens, the later tokens first: a half of S in registers, its maximum,
+        // its weights.  P overlays the second half of S: its columns 96..127 hold the weights of
+        // tokens 64..127 (S is in registers by then), 64..95 those of tokens 0..63.
 #pragma unroll 1
-            for (int i = 0; i < D; i += 16) {
-              uint32_t o[16];
-              tmem_ld16(t_o + i, o);
-              tmem_wait_ld16(o);
+        for (int half = 1; half >= 0; --half) {
+          if (active) {
+            float x0[32], x1[32];
+            tmem_ld32(t_s + half * 64, reinterpret_cast<uint32_t*>(x0));
+            tmem_ld32(t_s + half * 64 + 32, reinterpret_cast<uint32_t*>(x1));
+            tmem_wait_ld(reinterpret_cast<uint32_t*>(x0));
+            tmem_wait_ld(reinterpret_cast<uint32_t*>(x1));
+            if (base + half * 64 + 64 > whole) {  // some row of the warp ends inside the half
+              const int seen = limit - base - half * 64;
 #pragma unroll
-              for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-              tmem_st16(t_o + i, o);
+              for (int i = 0; i < 32; ++i) {
+                x0[i] = i < seen ? x0[i] : -INFINITY;
+                x1[i] = 32 + i < seen ? x1[i] : -INFINITY;
+              }
             }
+            float mx[4] = {x0[0], x0[1], x1[0], x1[1]};
+#pragma unroll
+            for (int i = 2; i < 32; i += 4) {
+              mx[0] = max3(mx[0], x0[i], x0[i + 1]);
+              mx[2] = max3(mx[2], x1[i], x1[i + 1]);
+              if (i + 2 < 32) {
+                mx[1] = max3(mx[1], x0[i + 2], x0[i + 3]);
+                mx[3] = max3(mx[3], x1[i + 2], x1[i + 3]);
+              }
+            }
+            const float m_new = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c);
+            if (__any_sync(~0u, m_new > m + kGrow)) {
+              const float f = m_new == m ? 1.0f : exp2f(m - m_new);
+              m = m_new;
+              l *= f;
+              // what O holds: the tiles before, and of this one the half that was handed over
+              if (j > 0 || half == 0) {
+                if (half == 0) {
+                  wait(&mi.o_half[w], n_s - 1);
+                  fence_after();
+                }
+#pragma unroll 1
+                for (int i = 0; i < D; i += 16) {
+                  uint32_t o[16];
+                  tmem_ld16(t_o + i, o);
+                  tmem_wait_ld16(o);
+#pragma unroll
+                  for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                  tmem_st16(t_o + i, o);
+                }
+              }
+            }
+            const float off = m == -INFINITY ? 0.0f : -m;
+            const uint64_t c2 = pack2(c, c), off2 = pack2(off, off);
+            uint64_t sum[2] = {0, 0};
+            auto weights = [&](int chunk, const float* x) {
+              uint32_t pk[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                float y0, y1, p0, p1;
+                unpack2(fma2(pack2(x[2 * i], x[2 * i + 1]), c2, off2), y0, y1);
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p0) : "f"(y0));
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p1) : "f"(y1));
+                sum[i & 1] = add2(sum[i & 1], pack2(p0, p1));
+                pk[i] = as_u32(__floats2half2_rn(p0, p1));
+              }
+              tmem_st16(t_s + 64 + half * 32 + chunk * 16, pk);
+            };
+            weights(0, x0);
+            weights(1, x1);
+            float l0, l1;
+            unpack2(add2(sum[0], sum[1]), l0, l1);
+            l += l0 + l1;
+            tmem_wait_st();
           }
-          const float off = m == -INFINITY ? 0.0f : -m;
-          const uint64_t c2 = pack2(c, c), off2 = pack2(off, off);
-          uint64_t sum[2] = {0, 0};
-          // P overlays the second half of S, whose chunks are in registers by now
-          auto weights = [&](int chunk, const float* x) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              float y0, y1, p0, p1;
-              unpack2(fma2(pack2(x[2 * i], x[2 * i + 1]), c2, off2), y0, y1);
-              asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p0) : "f"(y0));
-              asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p1) : "f"(y1));
-              sum[i & 1] = add2(sum[i & 1], pack2(p0, p1));
-              pk[i] = as_u32(__floats2half2_rn(p0, p1));
-            }
-            tmem_st16(t_s + 64 + chunk * 16, pk);
-          };
-          weights(2, x0);
-          ask(0, x0);
-          weights(3, x1);
-          tmem_wait_st();
           fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&mi.p_half[w]);  // the products with the second half may start
-          got(0, x0);
-          ask(1, x1);
-          weights(0, x0);
-          got(1, x1);
-          weights(1, x1);
-          float l0, l1;
-          unpack2(add2(sum[0], sum[1]), l0, l1);
-          l += l0 + l1;
-          tmem_wait_st();
-        };
-        if (active) {
-          if (base + kTile > whole) tile(Int<1>{});
-          else tile(Int<0>{});
-        } else if (lane == 0) {
-          mbar_arrive(&mi.p_half[w]);
+          if (lane == 0) mbar_arrive(half ? &mi.p_half[w] : &mi.p_full[w]);
         }
-        fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&mi.p_full[w]);
       }
 
       }
@@ -902,7 +904,7 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
       serial += it.tiles() > 0;
     }
   } else if (warp < 16) {
-    KNLP_REGISTERS("dec", 72);
+    KNLP_REGISTERS("dec", 80);
     if (warp < 12) produce<L, KM, D, 0>(p, sm, mi, n_items, warp - 8, lane);
     else produce<L, VM, D, 1>(p, sm, mi, n_items, warp - 12, lane);
   } else {
@@ -915,11 +917,14 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
       const uint32_t v_at = operand(smem_addr(sm + L::kRingAt), kTile * 128);
       const uint32_t idesc_s = product(kRows, kTile, raw_bf16, false);
       constexpr uint32_t idesc_o = product(kRows, D, false, true);
+      auto wait_warp = [&](uint64_t* x, uint32_t phase) { mbar_wait_warp(x, phase & 1, &mi.abort, p.status); };
+      const int n_all = uniform(n_items);
+      const uint32_t tm = uniform(tmem);
       uint32_t used = 0, n_q = 0, p_phase = 0;  // p_phase: bit w for stream w
       // S of stream w = Q tile qt x K tile, then the barriers that its end completes
       auto scores = [&](int w, int qt, uint32_t slot, bool last_use) {
         const uint32_t q = q_at + (qt * L::kTileBytes >> 4), kk = k_at + (slot * L::kTileBytes >> 4);
-        const uint32_t d = tmem + w * kTile;
+        const uint32_t d = tm + w * kTile;
         if (elect()) {
           auto step = [&](auto i) {
             constexpr int n = decltype(i)::value;
@@ -935,16 +940,19 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
       // O of stream w += P x V tile, second half of the tokens first, as P is written
       auto values = [&](int w, uint32_t slot, bool acc, bool last_use, bool last) {
         const uint32_t v = v_at + (slot * L::kTileBytes >> 4);
-        const uint32_t d = tmem + 256 + w * D, pr = tmem + w * kTile + 64;
+        const uint32_t d = tm + 256 + w * D, pr = tm + w * kTile + 64;
         auto step = [&](auto i, bool add) {
           constexpr int n = decltype(i)::value;
           mma_ts<n * 8, n * 2048 / 16>(d, pr, v, idesc_o, add);
         };
-        wait(&mi.p_half[w], p_phase >> w);
+        wait_warp(&mi.p_half[w], p_phase >> w);
         fence_after();
-        if (elect()) step(Int<4>{}, acc), step(Int<5>{}, true), step(Int<6>{}, true), step(Int<7>{}, true);
+        if (elect()) {
+          step(Int<4>{}, acc), step(Int<5>{}, true), step(Int<6>{}, true), step(Int<7>{}, true);
+          commit(&mi.o_half[w]);
+        }
         __syncwarp();
-        wait(&mi.p_full[w], p_phase >> w);
+        wait_warp(&mi.p_full[w], p_phase >> w);
         p_phase ^= 1u << w;
         fence_after();
         if (elect()) {
@@ -955,19 +963,19 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
         __syncwarp();
       };
       auto ready = [&](uint32_t x) {  // plane tile x of the ring
-        wait(&mi.ring_full[x % kRing], x / kRing);
+        wait_warp(&mi.ring_full[x % kRing], x / kRing);
         fence_after();
         return x % kRing;
       };
-      for (int k = blockIdx.x; k < n_items; k += gridDim.x) {
+      for (int k = blockIdx.x; k < n_all; k += gridDim.x) {
         const Item it(p, k);
-        const int n = it.tiles();
+        const int n = uniform(it.tiles());
         if (n == 0) continue;
-        wait(&mi.q_full, n_q++);
+        wait_warp(&mi.q_full, n_q++);
         fence_after();
         // Steps alternate between the streams: the output of one, then its next scores.  The
         // first two steps have scores only.  Of a pair, both streams use every K / V tile.
-        const bool pair = it.pair();
+        const bool pair = uniform(it.pair());
         const int steps = pair ? 2 * n : n;
         for (int i = -2; i < steps; ++i) {
           const int w = i & 1, j = pair ? i >> 1 : i, next = pair ? j + 1 : j + 2;
