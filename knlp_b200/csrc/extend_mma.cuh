@@ -11,16 +11,16 @@
 //
 // One CTA per SM (it owns all 512 TMEM columns), 20 warps whose registers are dealt out by
 // setmaxnreg (2 x 136 + 2 x 80 + 48 = 5 x 96 a lane):
-//   warps 0-3, 4-7   two softmax streams, a thread per query row.  An item of more than 128 rows
-//                    gives each stream its own 128 rows over the same K / V tiles; a smaller
-//                    one gives both streams the same rows and every other tile, and their
-//                    states are merged at the end.  Either way one stream's softmax runs under
-//                    the other's tensor work.
+//   warps 0-3, 4-7   two softmax streams, a thread per query row, 64 cached tokens at a time.  An
+//                    item of more than 128 rows gives each stream its own 128 rows over the
+//                    same K / V tiles; a smaller one gives both streams the same rows and a
+//                    half of every tile, and their states are merged at the end.  S has two
+//                    buffers per stream: the next scores are made under the softmax
 //   warps 8-11 (K),  dequantization: packed rows are staged with cp.async a few tiles ahead, turned
 //   12-15 (V)        into fp16 and written as swizzled tensor-core operands into a ring of three
 //                    tiles (K, V alternating).  An unquantized K tile is copied into the ring
-//   warp 16          (17-19 idle) issues the matrix products: S = Q K^T from shared memory,
-//                    O += P V with P read from TMEM, where it overlays S
+//   warps 16, 17     (18, 19 idle) issue a stream's products: S = Q K^T from shared memory,
+//                    O += P V with P read from TMEM, where it overlays its S
 //
 // Roundings, all chosen for the tensor cores' fp16 inputs: dequantized K and V, P and (from bf16)
 // Q are rounded to fp16, 2^-11 relative each; products accumulate in fp32, m, l and O are fp32.
@@ -42,7 +42,8 @@ namespace knlp {
 namespace extend {
 
 constexpr int kRows = 128;   // query rows of a stream
-constexpr int kTile = 128;   // cached tokens of a tile
+constexpr int kTile = 128;   // cached tokens of a K / V tile
+constexpr int kStep = 64;    // of a softmax step
 constexpr int kRing = 3;
 constexpr int kThreads = 20 * 32;
 constexpr int kMiscBytes = 2048;
@@ -130,7 +131,9 @@ struct Int {
 struct Misc {
   uint64_t ring_full[kRing];
   uint64_t ring_empty[2][kRing];  // a K tile, a V tile in the slot has been used
-  uint64_t q_full, s_full[2], p_half[2], p_full[2], o_half[2], o_full[2];
+  uint64_t q_full;
+  uint64_t s_full[2][2], p_full[2][2];  // [stream][buffer]
+  uint64_t o_step[2], o_full[2];        // a product with V, the item's last one, is done
   uint32_t tmem;
   int abort;
   float m[kRows], l[kRows];  // second stream's state when both serve the same rows
@@ -450,8 +453,8 @@ struct Item {
   }
   __device__ int tiles() const { return e.tile1 - e.tile0; }
   __device__ bool pair() const { return e.rows > kRows; }  // each stream has rows of its own
-  // tiles of stream w
-  __device__ int tiles_of(int w) const { return pair() ? tiles() : (tiles() + 1 - w) / 2; }
+  // steps of 64 tokens that each stream takes
+  __device__ int steps() const { return pair() ? 2 * tiles() : tiles(); }
 };
 
 // One plane's tiles (SIDE 0: K, 1: V), item after item, by a warpgroup: warp w copies and converts
@@ -608,13 +611,11 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
   const ExtendArgs& a = p.a;
 
   if (tid == 0) {
-    for (int i = 0; i < kRing; ++i) mbar_init(&mi.ring_full[i], 4), mbar_init(&mi.ring_empty[0][i], 1), mbar_init(&mi.ring_empty[1][i], 1);
+    for (int i = 0; i < kRing; ++i) mbar_init(&mi.ring_full[i], 4), mbar_init(&mi.ring_empty[0][i], 2), mbar_init(&mi.ring_empty[1][i], 2);
     mbar_init(&mi.q_full, 8);
     for (int w = 0; w < 2; ++w) {
-      mbar_init(&mi.s_full[w], 1);
-      mbar_init(&mi.p_half[w], 4);
-      mbar_init(&mi.p_full[w], 4);
-      mbar_init(&mi.o_half[w], 1);
+      for (int x = 0; x < 2; ++x) mbar_init(&mi.s_full[w][x], 1), mbar_init(&mi.p_full[w][x], 4);
+      mbar_init(&mi.o_step[w], 1);
       mbar_init(&mi.o_full[w], 1);
     }
     mi.abort = 0;
@@ -640,9 +641,9 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
     KNLP_REGISTERS("inc", 136);
     const int w = warp >> 2, row = tid & 127;  // row: of the stream's 128
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // the warp's 32 TMEM lanes
-    const uint32_t t_s = tmem + lanes + w * kTile, t_o = tmem + lanes + 256 + w * D;
+    const uint32_t t_s = tmem + lanes + w * 2 * kStep, t_o = tmem + lanes + 256 + w * D;
     const float c = a.scale * kLog2e;
-    uint32_t n_s = 0, n_o = 0;
+    uint32_t count = 0, n_o = 0;  // steps, items so far
     int serial = 0;
     // A thread's row of an item, derived anew behind the tiles: it would not fit the registers
     // beside S.
@@ -663,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
       float m = -INFINITY, l = 0.0f;
       {
       const Item it(p, k);
-      const int tiles = it.tiles_of(w);
+      const int steps = it.steps();
       const Row rw(p, it, w, row);
       const int limit = rw.limit;
       const bool active = rw.active;
@@ -706,38 +707,36 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
       __syncwarp();
       if (it.tiles() && lane == 0) mbar_arrive(&mi.q_full);
 
-      const int step = it.pair() ? kTile : 2 * kTile;
-      int base = (it.e.tile0 + (it.pair() ? 0 : w)) * kTile;
-      for (int j = 0; j < tiles; ++j, base += step) {
-        wait(&mi.s_full[w], n_s++);
-        fence_after();
-        // Two halves of 64 tokens, the later tokens first: a half of S in registers, its maximum,
-        // its weights.  P overlays the second half of S: its columns 96..127 hold the weights of
-        // tokens 64..127 (S is in registers by then), 64..95 those of tokens 0..63.
+      const int ahead = it.pair() ? kStep : kTile;
+      int base = it.e.tile0 * kTile + (it.pair() ? 0 : w * kStep);
 #pragma unroll 1
-        for (int half = 1; half >= 0; --half) {
+      for (int i = 0; i < steps; ++i, ++count, base += ahead) {
+        const uint32_t t_b = t_s + (count & 1) * kStep;
+        wait(&mi.s_full[w][count & 1], count >> 1);
+        fence_after();
+        {
           if (active) {
             float x0[32], x1[32];
-            tmem_ld32(t_s + half * 64, reinterpret_cast<uint32_t*>(x0));
-            tmem_ld32(t_s + half * 64 + 32, reinterpret_cast<uint32_t*>(x1));
+            tmem_ld32(t_b, reinterpret_cast<uint32_t*>(x0));
+            tmem_ld32(t_b + 32, reinterpret_cast<uint32_t*>(x1));
             tmem_wait_ld(reinterpret_cast<uint32_t*>(x0));
             tmem_wait_ld(reinterpret_cast<uint32_t*>(x1));
-            if (base + half * 64 + 64 > whole) {  // some row of the warp ends inside the half
-              const int seen = limit - base - half * 64;
+            if (base + kStep > whole) {  // some row of the warp ends inside the step
+              const int seen = limit - base;
 #pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                x0[i] = i < seen ? x0[i] : -INFINITY;
-                x1[i] = 32 + i < seen ? x1[i] : -INFINITY;
+              for (int x = 0; x < 32; ++x) {
+                x0[x] = x < seen ? x0[x] : -INFINITY;
+                x1[x] = 32 + x < seen ? x1[x] : -INFINITY;
               }
             }
             float mx[4] = {x0[0], x0[1], x1[0], x1[1]};
 #pragma unroll
-            for (int i = 2; i < 32; i += 4) {
-              mx[0] = max3(mx[0], x0[i], x0[i + 1]);
-              mx[2] = max3(mx[2], x1[i], x1[i + 1]);
-              if (i + 2 < 32) {
-                mx[1] = max3(mx[1], x0[i + 2], x0[i + 3]);
-                mx[3] = max3(mx[3], x1[i + 2], x1[i + 3]);
+            for (int x = 2; x < 32; x += 4) {
+              mx[0] = max3(mx[0], x0[x], x0[x + 1]);
+              mx[2] = max3(mx[2], x1[x], x1[x + 1]);
+              if (x + 2 < 32) {
+                mx[1] = max3(mx[1], x0[x + 2], x0[x + 3]);
+                mx[3] = max3(mx[3], x1[x + 2], x1[x + 3]);
               }
             }
             const float m_new = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c);
@@ -745,20 +744,17 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
               const float f = m_new == m ? 1.0f : exp2f(m - m_new);
               m = m_new;
               l *= f;
-              // what O holds: the tiles before, and of this one the half that was handed over
-              if (j > 0 || half == 0) {
-                if (half == 0) {
-                  wait(&mi.o_half[w], n_s - 1);
-                  fence_after();
-                }
+              if (i > 0) {  // O has the steps before, once the last product is done
+                wait(&mi.o_step[w], count - 1);
+                fence_after();
 #pragma unroll 1
-                for (int i = 0; i < D; i += 16) {
+                for (int col = 0; col < D; col += 16) {
                   uint32_t o[16];
-                  tmem_ld16(t_o + i, o);
+                  tmem_ld16(t_o + col, o);
                   tmem_wait_ld16(o);
 #pragma unroll
                   for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-                  tmem_st16(t_o + i, o);
+                  tmem_st16(t_o + col, o);
                 }
               }
             }
@@ -768,15 +764,15 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
             auto weights = [&](int chunk, const float* x) {
               uint32_t pk[16];
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
+              for (int e = 0; e < 16; ++e) {
                 float y0, y1, p0, p1;
-                unpack2(fma2(pack2(x[2 * i], x[2 * i + 1]), c2, off2), y0, y1);
+                unpack2(fma2(pack2(x[2 * e], x[2 * e + 1]), c2, off2), y0, y1);
                 asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p0) : "f"(y0));
                 asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p1) : "f"(y1));
-                sum[i & 1] = add2(sum[i & 1], pack2(p0, p1));
-                pk[i] = as_u32(__floats2half2_rn(p0, p1));
+                sum[e & 1] = add2(sum[e & 1], pack2(p0, p1));
+                pk[e] = as_u32(__floats2half2_rn(p0, p1));
               }
-              tmem_st16(t_s + 64 + half * 32 + chunk * 16, pk);
+              tmem_st16(t_b + chunk * 16, pk);  // P overlays S, which is in registers by now
             };
             weights(0, x0);
             weights(1, x1);
@@ -787,21 +783,21 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
           }
           fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(half ? &mi.p_half[w] : &mi.p_full[w]);
+          if (lane == 0) mbar_arrive(&mi.p_full[w][count & 1]);
         }
       }
 
       }
       // ---- epilogue
       const Item it(p, k);
-      const int tiles = it.tiles_of(w);
+      const int steps = it.steps();
       const auto [local, flat, tok, limit, valid, active] = Row(p, it, w, row);
-      if (tiles) {
+      if (steps) {
         wait(&mi.o_full[w], n_o++);
         fence_after();
       }
       float* swap = reinterpret_cast<float*>(sm + L::kQ);  // [column][row] of the second stream
-      const bool merge = !it.pair() && it.tiles_of(1) > 0;
+      const bool merge = !it.pair() && steps > 0;
       if (merge && w == 1) {
         if (active) {
 #pragma unroll
@@ -837,7 +833,7 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
 #pragma unroll
         for (int i = 0; i < D; i += 32) {
           float o[32];
-          if (tiles) {
+          if (steps) {
             tmem_ld32(t_o + i, reinterpret_cast<uint32_t*>(o));
             tmem_wait_ld(reinterpret_cast<uint32_t*>(o));
           } else {
@@ -910,21 +906,23 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
   } else {
     // ---------------------------------------------------------------- matrix products
     KNLP_REGISTERS("dec", 48);
-    if (warp == 16) {
-      // The whole warp follows the items and waits; one lane issues.
+    if (warp < 18) {
+      // A warp per stream; all of it follows the items and waits, one lane issues.
+      const int w = warp - 16;
       const uint32_t q_at = operand(smem_addr(sm + L::kQ), 16);
       const uint32_t k_at = operand(smem_addr(sm + L::kRingAt), 16);
       const uint32_t v_at = operand(smem_addr(sm + L::kRingAt), kTile * 128);
-      const uint32_t idesc_s = product(kRows, kTile, raw_bf16, false);
+      const uint32_t idesc_s = product(kRows, kStep, raw_bf16, false);
       constexpr uint32_t idesc_o = product(kRows, D, false, true);
       auto wait_warp = [&](uint64_t* x, uint32_t phase) { mbar_wait_warp(x, phase & 1, &mi.abort, p.status); };
       const int n_all = uniform(n_items);
       const uint32_t tm = uniform(tmem);
-      uint32_t used = 0, n_q = 0, p_phase = 0;  // p_phase: bit w for stream w
-      // S of stream w = Q tile qt x K tile, then the barriers that its end completes
-      auto scores = [&](int w, int qt, uint32_t slot, bool last_use) {
-        const uint32_t q = q_at + (qt * L::kTileBytes >> 4), kk = k_at + (slot * L::kTileBytes >> 4);
-        const uint32_t d = tm + w * kTile;
+      uint32_t used = 0, n_q = 0, count = 0;
+      // S buffer b = Q tile qt x half a K tile
+      auto scores = [&](int b, int qt, uint32_t slot, int half, bool last_use) {
+        const uint32_t q = q_at + (qt * L::kTileBytes >> 4);
+        const uint32_t kk = k_at + (slot * L::kTileBytes >> 4) + half * (kStep * 128 >> 4);
+        const uint32_t d = tm + (w * 2 + b) * kStep;
         if (elect()) {
           auto step = [&](auto i) {
             constexpr int n = decltype(i)::value;
@@ -932,31 +930,22 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
           };
           step(Int<0>{}), step(Int<1>{}), step(Int<2>{}), step(Int<3>{});
           if constexpr (D == 128) step(Int<4>{}), step(Int<5>{}), step(Int<6>{}), step(Int<7>{});
-          commit(&mi.s_full[w]);
+          commit(&mi.s_full[w][b]);
           if (last_use) commit(&mi.ring_empty[0][slot]);
         }
         __syncwarp();
       };
-      // O of stream w += P x V tile, second half of the tokens first, as P is written
-      auto values = [&](int w, uint32_t slot, bool acc, bool last_use, bool last) {
-        const uint32_t v = v_at + (slot * L::kTileBytes >> 4);
-        const uint32_t d = tm + 256 + w * D, pr = tm + w * kTile + 64;
-        auto step = [&](auto i, bool add) {
-          constexpr int n = decltype(i)::value;
-          mma_ts<n * 8, n * 2048 / 16>(d, pr, v, idesc_o, add);
-        };
-        wait_warp(&mi.p_half[w], p_phase >> w);
-        fence_after();
+      // O (+)= P in buffer b x half a V tile
+      auto values = [&](int b, uint32_t slot, int half, bool acc, bool last_use, bool last) {
+        const uint32_t v = v_at + (slot * L::kTileBytes >> 4) + half * (kStep * 128 >> 4);
+        const uint32_t d = tm + 256 + w * D, pr = tm + (w * 2 + b) * kStep;
         if (elect()) {
-          step(Int<4>{}, acc), step(Int<5>{}, true), step(Int<6>{}, true), step(Int<7>{}, true);
-          commit(&mi.o_half[w]);
-        }
-        __syncwarp();
-        wait_warp(&mi.p_full[w], p_phase >> w);
-        p_phase ^= 1u << w;
-        fence_after();
-        if (elect()) {
-          step(Int<0>{}, true), step(Int<1>{}, true), step(Int<2>{}, true), step(Int<3>{}, true);
+          auto step = [&](auto i, bool add) {
+            constexpr int n = decltype(i)::value;
+            mma_ts<n * 8, n * 2048 / 16>(d, pr, v, idesc_o, add);
+          };
+          step(Int<0>{}, acc), step(Int<1>{}, true), step(Int<2>{}, true), step(Int<3>{}, true);
+          commit(&mi.o_step[w]);
           if (last_use) commit(&mi.ring_empty[1][slot]);
           if (last) commit(&mi.o_full[w]);
         }
@@ -973,16 +962,25 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
         if (n == 0) continue;
         wait_warp(&mi.q_full, n_q++);
         fence_after();
-        // Steps alternate between the streams: the output of one, then its next scores.  The
-        // first two steps have scores only.  Of a pair, both streams use every K / V tile.
+        // Step i: its output, then the scores of step i + 2.  Of a pair both streams use the same
+        // half tiles, else each its half of every tile.
         const bool pair = uniform(it.pair());
         const int steps = pair ? 2 * n : n;
         for (int i = -2; i < steps; ++i) {
-          const int w = i & 1, j = pair ? i >> 1 : i, next = pair ? j + 1 : j + 2;
-          const bool last_use = !pair || w;
-          if (i >= 0) values(w, ready(used + 2 * j + 1), pair ? j > 0 : j > 1, last_use, next >= n);
-          if (next < n) scores(w, pair ? w : 0, ready(used + 2 * next), last_use);
+          if (i >= 0) {
+            const uint32_t slot = ready(used + 2 * (pair ? i >> 1 : i) + 1);
+            const int b = (count + i) & 1;
+            wait_warp(&mi.p_full[w][b], (count + i) >> 1);
+            fence_after();
+            values(b, slot, pair ? i & 1 : w, i > 0, !pair || (i & 1), i + 1 == steps);
+          }
+          const int x = i + 2;
+          if (x < steps) {
+            const uint32_t slot = ready(used + 2 * (pair ? x >> 1 : x));
+            scores((count + x) & 1, pair ? w : 0, slot, pair ? x & 1 : w, !pair || (x & 1));
+          }
         }
+        count += steps;
         used += 2 * n;
       }
     }
