@@ -119,9 +119,10 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(StepArgs a) {
       return lo;
     };
     // fresh table entries, in runs of kThreads dealt to the blocks in turn
-    for (int64_t run = fresh_base / kThreads * kThreads; run < fresh_base + all_f; run += kThreads) {
-      if (run / kThreads % gridDim.x != blockIdx.x) continue;
-      const int64_t j = run + tid;
+    const int64_t first_run = fresh_base / kThreads;
+    const unsigned skip = (blockIdx.x + gridDim.x - static_cast<unsigned>(first_run % gridDim.x)) % gridDim.x;
+    for (int64_t run = first_run + skip; run * kThreads < fresh_base + all_f; run += gridDim.x) {
+      const int64_t j = run * kThreads + tid;
       if (j < fresh_base || j >= fresh_base + all_f) continue;
       const int v = static_cast<int>(j - fresh_base);
       const int i = find(s_fresh, v);
