@@ -128,21 +128,6 @@ struct Int {
   static constexpr int value = N;
 };
 
-struct Misc {
-  uint64_t ring_full[kRing];
-  uint64_t ring_empty[2][kRing];  // a K tile, a V tile in the slot has been used
-  uint64_t q_full;
-  uint64_t s_full[2][2], p_full[2][2];  // [stream][buffer]
-  uint64_t o_step[2], o_full[2];        // a product with V, the item's last one, is done
-  uint32_t tmem;
-  int abort;
-  float m[kRows], l[kRows];  // second stream's state when both serve the same rows
-  // tokens with a scale or zero-point that is not finite, by item: (token, mask of groups)
-  int bad_count[kBadLists];
-  int2 bad[kBadLists][kBadMost + 1];
-};
-static_assert(sizeof(Misc) <= kMiscBytes, "");
-
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
@@ -437,6 +422,25 @@ __device__ __forceinline__ int not_finite(const char* stage, int row) {
   return mask;
 }
 
+// Eight elements of a query row as the product with a K operand of mode KM wants them: fp16 beside
+// dequantized K, in the order of the nibbles beside 4-bit K.
+template <int KM>
+__device__ __forceinline__ uint4 query_operand(uint4 v, int dtype) {
+  if constexpr (KM != kRaw) {
+    if (dtype == KNLP_BF16) {
+      uint32_t* u = &v.x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        u[j] = as_u32(__floats2half2_rn(__uint_as_float(u[j] << 16), __uint_as_float(u[j] & 0xffff0000u)));
+    }
+  }
+  if constexpr (KM == KNLP_KV_INT4_SYM || KM == KNLP_KV_INT4_ASYM) {
+    v = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
+                   __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+  }
+  return v;
+}
+
 // Geometry of an item that every role derives for itself.
 struct Item {
   Entry e;
@@ -457,31 +461,35 @@ struct Item {
   __device__ int steps() const { return pair() ? 2 * tiles() : tiles(); }
 };
 
-// One plane's tiles (SIDE 0: K, 1: V), item after item, by a warpgroup: warp w copies and converts
-// rows 32 w .. 32 w + 31 of every tile, a lane converts one row, and only lanes of the same
-// warp read what a lane has copied.  The block of a row is looked up a tile before it is needed.
-template <class L, int MODE, int D, int SIDE>
-__device__ __forceinline__ void produce(const Params& p, char* sm, Misc& mi, int n_items, int w,
-                                        int lane) {
+// Copies of one plane's tiles by a warpgroup, item after item: warp w copies rows 32 w .. 32 w + 31
+// of every tile, a lane looks up one row's block, a tile before it is needed.  PHASE >= 0: only
+// every other tile, counted over all items.
+template <int MODE, int D, int SIDE, int PHASE>
+struct Copies {
   using T = PlaneTile<MODE, D>;
-  constexpr int kStages = SIDE ? L::kStagesV : L::kStagesK;
-  constexpr int kAhead = kStages ? kStages : 1;
-  const ExtendArgs& a = p.a;
-  const Plane& pl = SIDE ? a.v : a.k;
-  char* const stages = sm + (SIDE ? L::kStageV : L::kStageK);
-  const int row = w * 32 + lane;
-
-  // the next tile to copy: its row of this lane
+  const Params& p;
+  const Plane& pl;
+  const int n_items, w, lane;
   int k = blockIdx.x, tile = 0, tile1 = 0, len = 0, block = 0, off = 0;
+  uint32_t count = 0;  // tiles of the items so far
   const int32_t* table = nullptr;
   const char* head_codes = nullptr;
   int64_t head_scales = 0, head_zeros = 0;
-  bool there = false;
-  auto look_up = [&]() -> bool {
-    while (tile == tile1 && k < n_items) {  // the first tile of the next item that has any
+  bool there = false, pending;  // pending: a tile is looked up
+
+  __device__ __forceinline__ Copies(const Params& p_, int n_items_, int w_, int lane_)
+      : p(p_), pl(SIDE ? p_.a.v : p_.a.k), n_items(n_items_), w(w_), lane(lane_) {
+    pending = look_up();
+  }
+  __device__ __forceinline__ bool look_up() {
+    while (tile >= tile1 && k < n_items) {  // the first tile of the next item that has any
       const Item it(p, k);
       tile = it.e.tile0, tile1 = it.e.tile1, len = it.len;
-      table = a.block_table + it.e.seq * a.bt_stride;
+      if constexpr (PHASE >= 0) {
+        tile += (count & 1) != PHASE;
+        count += it.tiles();
+      }
+      table = p.a.block_table + it.e.seq * p.a.bt_stride;
       head_codes = reinterpret_cast<const char*>(pl.codes) + it.head * pl.cs[2];
       if constexpr (T::kQuant) {
         head_scales = it.head * pl.ss[2];
@@ -489,19 +497,21 @@ __device__ __forceinline__ void produce(const Params& p, char* sm, Misc& mi, int
       }
       k += gridDim.x;
     }
-    if (tile == tile1) return false;
-    const int t = tile * kTile + row;
+    if (tile >= tile1) return false;
+    const int t = tile * kTile + w * 32 + lane;
     there = t < len;
-    const int e = p.block_shift >= 0 ? t >> p.block_shift : t / a.block_size;
-    off = t - e * a.block_size;
+    const int e = p.block_shift >= 0 ? t >> p.block_shift : t / p.a.block_size;
+    off = t - e * p.a.block_size;
     block = there ? table[e] : 0;
-    ++tile;
+    tile += PHASE >= 0 ? 2 : 1;
     return true;
-  };
-  bool pending = look_up();  // copies run ahead of the conversion, over the items' ends
-  auto copy = [&](char* dst) {  // the looked-up tile, if any
+  }
+  // The looked-up tile to `dst`, a stage (or the operand itself, unquantized), as one group of
+  // asynchronous copies; then the look-up of the next.
+  __device__ __forceinline__ void next(char* dst) {
     if (pending) {
-      const int64_t b = block < 0 ? 0 : block >= a.num_blocks ? a.num_blocks - 1 : block;
+      const int row = w * 32 + lane;
+      const int64_t b = block < 0 ? 0 : block >= p.a.num_blocks ? p.a.num_blocks - 1 : block;
       const char* src = there ? head_codes + b * pl.cs[0] + off * pl.cs[1] : nullptr;
       const uint32_t lo = static_cast<uint32_t>(reinterpret_cast<uint64_t>(src));
       const uint32_t hi = static_cast<uint32_t>(reinterpret_cast<uint64_t>(src) >> 32);
@@ -526,13 +536,70 @@ __device__ __forceinline__ void produce(const Params& p, char* sm, Misc& mi, int
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-  if constexpr (kStages > 0) {
-    for (int i = 0; i < kStages; ++i) {
-      copy(stages + i * T::kBytes);
-      pending = pending && look_up();
+    pending = pending && look_up();
+  }
+};
+
+// Tokens of an item whose V is not finite in some groups.  Such a value would reach rows that do
+// not attend to its token (as 0 x NaN): the groups are zeroed in the stage and noted, and the
+// rows that do attend to the token are made NaN at the end.
+struct BadList {
+  int count;
+  int2 at[kBadMost + 1];  // (token, mask of groups); the last one: from this token on
+  __device__ __forceinline__ void clear() {
+    count = 0;
+    at[kBadMost] = make_int2(0x7fffffff, 0);
+  }
+  template <int MODE, int D>
+  __device__ __forceinline__ void note(char* stage, int row, int token) {
+    using T = PlaneTile<MODE, D>;
+    const int bad = not_finite<MODE, D>(stage, row);
+    for (int g = 0; g < D / 32; ++g) {
+      if (!(bad >> g & 1)) continue;
+      *reinterpret_cast<uint16_t*>(stage + T::kScaleAt + row * T::kScaleBytes + 2 * g) = 0;
+      if constexpr (T::kBytes > T::kZeroAt)
+        *reinterpret_cast<uint16_t*>(stage + T::kZeroAt + row * T::kScaleBytes + 2 * g) = 0;
+    }
+    const int i = atomicAdd(&count, 1);
+    if (i < kBadMost) {
+      at[i] = make_int2(token, bad);
+    } else {  // more than the list holds
+      atomicMin(&at[kBadMost].x, token);
+      atomicOr(&at[kBadMost].y, bad);
     }
   }
+  // whether a row that attends to `limit` tokens sees such a value in the group
+  __device__ __forceinline__ bool hits(int limit, int group) const {
+    bool hit = false;
+    for (int i = 0; i < min(count, kBadMost + 1); ++i) hit |= limit > at[i].x && (at[i].y >> group & 1);
+    return hit;
+  }
+};
+
+struct Misc {
+  uint64_t ring_full[kRing];
+  uint64_t ring_empty[2][kRing];  // a K tile, a V tile in the slot has been used
+  uint64_t q_full;
+  uint64_t s_full[2][2], p_full[2][2];  // [stream][buffer]
+  uint64_t o_step[2], o_full[2];        // a product with V, the item's last one, is done
+  uint32_t tmem;
+  int abort;
+  float m[kRows], l[kRows];  // second stream's state when both serve the same rows
+  BadList bad[kBadLists];    // by item
+};
+static_assert(sizeof(Misc) <= kMiscBytes, "");
+
+// One plane's tiles (SIDE 0: K, 1: V) by a warpgroup: a lane converts one row of every tile, and
+// only lanes of the same warp read what a lane has copied.
+template <class L, int MODE, int D, int SIDE>
+__device__ __forceinline__ void produce(const Params& p, char* sm, Misc& mi, int n_items, int w,
+                                        int lane) {
+  using T = PlaneTile<MODE, D>;
+  constexpr int kStages = SIDE ? L::kStagesV : L::kStagesK;
+  char* const stages = sm + (SIDE ? L::kStageV : L::kStageK);
+  const int row = w * 32 + lane;
+  Copies<MODE, D, SIDE, -1> copies(p, n_items, w, lane);
+  for (int i = 0; i < kStages; ++i) copies.next(stages + i * T::kBytes);
   uint32_t done = SIDE, stage = 0;  // done: number of the plane tile in the ring's order
   // The slot's use before this one, always the other plane's, has to be over.
   auto wait_empty = [&]() {
@@ -543,46 +610,23 @@ __device__ __forceinline__ void produce(const Params& p, char* sm, Misc& mi, int
   for (int ki = blockIdx.x; ki < n_items; ki += gridDim.x) {
     const Item it(p, ki);
     if (it.tiles() == 0) continue;
-    if constexpr (SIDE == 1 && T::kQuant) {
-      if (row == 0) {
-        mi.bad_count[serial % kBadLists] = 0;
-        mi.bad[serial % kBadLists][kBadMost] = make_int2(0x7fffffff, 0);
-      }
+    BadList& bad = mi.bad[serial % kBadLists];
+    if constexpr (SIDE == 1) {
+      if (row == 0) bad.clear();
       asm volatile("bar.sync 3, 128;" ::: "memory");
     }
     for (int j = 0; j < it.tiles(); ++j, done += 2) {
       char* const to = sm + L::kRingAt + done % kRing * L::kTileBytes;
-        if constexpr (kStages == 0) {
+      if constexpr (kStages == 0) {
         wait_empty();
-        copy(to);
-        pending = pending && look_up();
+        copies.next(to);
         asm volatile("cp.async.wait_group 0;" ::: "memory");
       } else {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
         __syncwarp();
         char* const from = stages + stage * T::kBytes;
         if constexpr (SIDE == 1) {
-          // A value that is not finite would reach rows that do not attend to its token (as
-          // 0 x NaN): such groups are zeroed here and noted, and the rows that do attend to
-          // the token are made NaN at the end.
-          if (any_not_finite<MODE, D>(from, row)) {
-            const int bad = not_finite<MODE, D>(from, row);
-            for (int g = 0; g < D / 32; ++g) {
-              if (!(bad >> g & 1)) continue;
-              *reinterpret_cast<uint16_t*>(from + T::kScaleAt + row * T::kScaleBytes + 2 * g) = 0;
-              if constexpr (T::kBytes > T::kZeroAt)
-                *reinterpret_cast<uint16_t*>(from + T::kZeroAt + row * T::kScaleBytes + 2 * g) = 0;
-            }
-            const int token = (it.e.tile0 + j) * kTile + row;
-            const int at = atomicAdd(&mi.bad_count[serial % kBadLists], 1);
-            int2* list = mi.bad[serial % kBadLists];
-            if (at < kBadMost) {
-              list[at] = make_int2(token, bad);
-            } else {  // more than the list holds: from the first of them on, all their groups
-              atomicMin(&list[kBadMost].x, token);
-              atomicOr(&list[kBadMost].y, bad);
-            }
-          }
+          if (any_not_finite<MODE, D>(from, row)) bad.note<MODE, D>(from, row, (it.e.tile0 + j) * kTile + row);
         }
         wait_empty();
         dequantize_row<MODE, D>(from, to, row);
@@ -591,8 +635,7 @@ __device__ __forceinline__ void produce(const Params& p, char* sm, Misc& mi, int
       __syncwarp();
       if (lane == 0) mbar_arrive(&mi.ring_full[done % kRing]);
       if constexpr (kStages > 0) {
-        copy(stages + stage * T::kBytes);
-        pending = pending && look_up();
+        copies.next(stages + stage * T::kBytes);
         stage = stage + 1 == kStages ? 0 : stage + 1;
       }
     }
@@ -621,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
     mi.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (tid < kBadLists) mi.bad_count[tid] = 0;
+  if (tid < kBadLists) mi.bad[tid].clear();
   if (warp == 16) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&mi.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -687,20 +730,8 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
                                 (static_cast<int64_t>(it.head) * p.rep + (f - t * p.rep)) * a.q_stride[1];
             v = reinterpret_cast<const uint4*>(static_cast<const char*>(a.q) + 2 * off)[chunk];
           }
-          if constexpr (KM != kRaw) {
-            if (a.q_dtype == KNLP_BF16) {
-              uint32_t* u = &v.x;
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                u[j] = as_u32(__floats2half2_rn(__uint_as_float(u[j] << 16), __uint_as_float(u[j] & 0xffff0000u)));
-            }
-          }
-          if constexpr (KM == KNLP_KV_INT4_SYM || KM == KNLP_KV_INT4_ASYM) {
-            v = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
-                           __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
-          }
           *reinterpret_cast<uint4*>(q + (chunk >> 3) * (kRows * 128) + r * 128 +
-                                    (((chunk & 7) ^ (r & 7)) << 4)) = v;
+                                    (((chunk & 7) ^ (r & 7)) << 4)) = query_operand<KM>(v, a.q_dtype);
         }
         fence_smem();
       }
@@ -825,7 +856,7 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
         }
         const bool direct = it.e.part < 0;
         const float inv = !direct ? 1.0f : l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
-        const int bad = mi.bad_count[serial % kBadLists];
+        const BadList& bad = mi.bad[serial % kBadLists];
         const int h = flat - tok * p.rep;
         const int64_t out_row = (static_cast<int64_t>(it.first) + tok) * a.n_q_heads + it.head * p.rep + h;
         float* part = direct ? nullptr
@@ -845,14 +876,9 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
             if (merge) o[x] = o[x] * f0 + swap[(i + x) * kRows + row] * f1;
             o[x] *= inv;
           }
-          if (bad) {  // never in a healthy cache
-            for (int b = 0; b < min(bad, kBadMost + 1); ++b) {
-              const int2 t = mi.bad[serial % kBadLists][b];
-              if (limit > t.x && (t.y >> (i / 32) & 1)) {
+          if (bad.count && bad.hits(limit, i / 32)) {  // never in a healthy cache
 #pragma unroll
-                for (int x = 0; x < 32; ++x) o[x] = NAN;
-              }
-            }
+            for (int x = 0; x < 32; ++x) o[x] = NAN;
           }
           if (!valid) continue;
           float v[32];  // in the order of the head dimension
@@ -994,47 +1020,7 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-// One pair of plane modes, both head dimensions.
-template <int KM, int VM>
-int launch_extend_pair(const Params& p, int grid, cudaStream_t st);
-
-template <int KM, int VM, int D>
-int launch_extend_one(const Params& p, int grid, cudaStream_t st) {
-  using L = Layout<KM, VM, D>;
-  auto* fn = extend_mma_kernel<KM, VM, D>;
-  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes) != cudaSuccess) {
-    cudaGetLastError();
-    return KNLP_ERR_NO_DEVICE;
-  }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = L::kBytes;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, fn, p) != cudaSuccess) {
-    cudaGetLastError();
-    return KNLP_ERR_LAUNCH;
-  }
-  return KNLP_OK;
-}
-
 #undef KNLP_REGISTERS
-
-#define KNLP_EXTEND_PAIR(KM, VM)                                                   \
-  namespace knlp {                                                                 \
-  namespace extend {                                                               \
-  template <>                                                                      \
-  int launch_extend_pair<KM, VM>(const Params& p, int grid, cudaStream_t st) {     \
-    return p.a.head_dim == 64 ? launch_extend_one<KM, VM, 64>(p, grid, st)         \
-                              : launch_extend_one<KM, VM, 128>(p, grid, st);       \
-  }                                                                                \
-  }                                                                                \
-  }
 
 }  // namespace extend
 }  // namespace knlp

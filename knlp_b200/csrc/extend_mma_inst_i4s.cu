@@ -1,4 +1,4 @@
 // Tensor-core extend attention: instantiation for one pair of plane modes.
-#include "extend_mma.cuh"
+#include "extend_launch.cuh"
 
 KNLP_EXTEND_PAIR(KNLP_KV_INT4_SYM, KNLP_KV_INT4_SYM)

@@ -2,14 +2,15 @@
 // the kernel that merges the pieces of split rows.
 //
 // Work: the packed query rows (token x group head) of a sequence are cut into tiles of 256, each
-// with the cached tokens it can see; a tile's range of cached tokens may be cut into pieces that
-// different CTAs serve and a last kernel merges.  The lengths live on the GPU, so a block of one
-// CTA plans there: it counts the tiles, weighs a dozen piece lengths by the rounds that the
+// with the cached tokens it can see; a last tile of at most 32 rows goes to the kernel for few
+// rows (extend_few.cuh), the others to the one for many (extend_mma.cuh).  A tile's range of cached
+// tokens may be cut into pieces that different CTAs serve and a last kernel merges.  The lengths
+// live on the GPU, so a block per kernel plans there: it counts the tiles, weighs a dozen piece lengths by the rounds that the
 // resulting items need on the machine, and writes the list of pieces.  Items are (piece, kv head),
 // heads innermost: the CTAs that serve the heads of one piece run at the same time and share the
 // 32-byte sectors in which the scales of several heads lie.
 
-#include "extend_mma.cuh"
+#include "extend_launch.cuh"
 
 namespace knlp {
 namespace extend {
@@ -22,17 +23,19 @@ constexpr int kMaxRows = 2 * kRows;
 // (query in, result out, an empty pipeline at both ends), and of the merging launch.
 constexpr float kItemCost = 4.0f, kMergeCost = 5.0f;
 
-int64_t tiles_bound(int n_seqs, int64_t rows) { return rows / kMaxRows + n_seqs; }
-int64_t entries_bound(int n_seqs, int64_t rows, int heads, int n_sms) {
-  return 2 * tiles_bound(n_seqs, rows) + 16 * static_cast<int64_t>(n_sms) / heads + 2;
-}
-// Partial rows: enough to cut every row once, within a bound of a few tiles per SM and more than
-// that only for large inputs.
-int64_t parts_bound(int n_tokens, int n_q_heads, int n_sms) {
-  const int64_t rows = static_cast<int64_t>(n_tokens) * n_q_heads;
-  const int64_t most = static_cast<int64_t>(n_sms) * 3 * kMaxRows;
-  return rows * 64 < most ? rows * 64 : most;
-}
+// Sizes of a kernel's lists.  few: the tiles of at most 32 rows, one per sequence at most.
+struct Bounds {
+  int64_t tiles, entries, parts;  // parts: rows of partial results
+  Bounds(bool few, int n_seqs, int n_tokens, int n_q_heads, int n_kv_heads, int n_sms) {
+    const int64_t rows = static_cast<int64_t>(n_tokens) * (n_q_heads / n_kv_heads);
+    tiles = few ? n_seqs : rows / kMaxRows + n_seqs;
+    entries = 2 * tiles + 16 * static_cast<int64_t>(n_sms) / n_kv_heads + 2;
+    // every row in pieces, up to a few tiles per SM
+    const int64_t all = static_cast<int64_t>(n_tokens) * n_q_heads * 64;
+    const int64_t most = static_cast<int64_t>(n_sms) * (few ? 8 * few::kFewRows : 3 * kMaxRows);
+    parts = all < most ? all : most;
+  }
+};
 
 struct Tile {
   int seq, row0, rows, kv;  // kv: tiles of cached tokens
@@ -44,7 +47,7 @@ struct Tile {
   }
 };
 
-__device__ Tile tile_at(const ExtendArgs& a, int rep, const int* base, int t) {
+__device__ Tile tile_at(const ExtendArgs& a, bool few_rows, int rep, const int* base, int t) {
   int lo = 0, hi = a.n_seqs - 1;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
@@ -54,12 +57,18 @@ __device__ Tile tile_at(const ExtendArgs& a, int rep, const int* base, int t) {
   const int n = extend_rows(a, lo, &first), len = extend_length(a, lo);
   Tile x;
   x.seq = lo;
-  x.row0 = (t - base[lo]) * kMaxRows;
+  x.row0 = few_rows ? n * rep / kMaxRows * kMaxRows : (t - base[lo]) * kMaxRows;
   x.rows = min(kMaxRows, n * rep - x.row0);
   const int last = (x.row0 + x.rows - 1) / rep;
   const int seen = a.causal ? max(min(a.seq_lens[lo] - n + last + 1, len), 0) : len;
   x.kv = (seen + kTile - 1) / kTile;
   return x;
+}
+// Tiles of a sequence with that many rows.
+__device__ int tiles_of(bool few_rows, int64_t rows) {
+  const int rest = static_cast<int>(rows % kMaxRows);
+  const bool few = rest > 0 && rest <= few::kFewRows;
+  return few_rows ? few : static_cast<int>(rows / kMaxRows) + (rest > 0 && !few);
 }
 
 // Exclusive prefix sums of N values over the block, and their totals.
@@ -92,10 +101,22 @@ __device__ void scan(int (&v)[N], int (&total)[N], int (*sh)[kPlanThreads / 32])
   }
 }
 
+// A kernel's lists in the workspace.
+struct Lists {
+  int max_entries, max_tiles;
+  int64_t max_parts;
+  int* base;  // first tile of each sequence
+  Plan* plan;
+  Entry* entries;
+  Split* splits;
+};
+
 __global__ void __launch_bounds__(kPlanThreads)
-extend_plan_kernel(const __grid_constant__ ExtendArgs a, int rep, int n_ctas, int max_entries,
-                   int max_splits, int64_t max_parts, int* base, Plan* plan, Entry* entries,
-                   Split* splits) {
+extend_plan_kernel(const __grid_constant__ ExtendArgs a, int rep, int n_ctas, const __grid_constant__ Lists many,
+                   const __grid_constant__ Lists few) {
+  const bool few_rows = blockIdx.x;  // a block per kernel
+  const Lists& to = few_rows ? few : many;
+  int* const base = to.base;
   __shared__ int sh[4][kPlanThreads / 32];
   __shared__ float sh_cost[kCandidates], sh_piece[kCandidates];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -106,8 +127,7 @@ extend_plan_kernel(const __grid_constant__ ExtendArgs a, int rep, int n_ctas, in
     const int s = s0 + tid;
     int first, v[1] = {0}, total[1];
     if (s < a.n_seqs) {
-      const int64_t r = static_cast<int64_t>(extend_rows(a, s, &first)) * rep;
-      v[0] = static_cast<int>((r + kMaxRows - 1) / kMaxRows);
+      v[0] = tiles_of(few_rows, static_cast<int64_t>(extend_rows(a, s, &first)) * rep);
     }
     scan(v, total, sh);
     if (s < a.n_seqs) base[s] = n_tiles + v[0];
@@ -115,10 +135,10 @@ extend_plan_kernel(const __grid_constant__ ExtendArgs a, int rep, int n_ctas, in
   }
   if (tid == 0) base[a.n_seqs] = n_tiles;
   __syncthreads();
-  n_tiles = min(n_tiles, max_splits);  // more only for offsets that are not ascending
+  n_tiles = min(n_tiles, to.max_tiles);  // more only for offsets that are not ascending
 
   float cost = 0.0f;
-  for (int t = tid; t < n_tiles; t += kPlanThreads) cost += tile_at(a, rep, base, t).cost();
+  for (int t = tid; t < n_tiles; t += kPlanThreads) cost += tile_at(a, few_rows, rep, base, t).cost();
 #pragma unroll
   for (int d = 16; d; d >>= 1) cost += __shfl_xor_sync(~0u, cost, d);
   if (lane == 0) sh_cost[warp] = cost;
@@ -134,7 +154,7 @@ extend_plan_kernel(const __grid_constant__ ExtendArgs a, int rep, int n_ctas, in
   int items = 0;
   int64_t parts = 0;
   for (int t = lane; t < n_tiles; t += 32) {
-    const Tile x = tile_at(a, rep, base, t);
+    const Tile x = tile_at(a, few_rows, rep, base, t);
     const int n = x.pieces(piece);
     items += n;
     worst = fmaxf(worst, x.cost() / n);
@@ -153,7 +173,7 @@ extend_plan_kernel(const __grid_constant__ ExtendArgs a, int rep, int n_ctas, in
     // writing and reading a partial row takes about 2e-3 of a unit on the whole machine
     float est = fmaxf(rounds * (items ? cost * heads / items + kItemCost : 0.0f), worst + kItemCost) +
                 (parts ? kMergeCost + 1e-3f * parts : 0.0f);
-    if (parts > max_parts) est = 1e30f;
+    if (parts > to.max_parts) est = 1e30f;
     if (warp == 0) est = fminf(est, 1e29f);  // always possible
     sh_cost[warp] = est;
     sh_piece[warp] = piece;
@@ -170,40 +190,42 @@ extend_plan_kernel(const __grid_constant__ ExtendArgs a, int rep, int n_ctas, in
     Tile x{};
     int n = 0;
     if (t < n_tiles) {
-      x = tile_at(a, rep, base, t);
+      x = tile_at(a, few_rows, rep, base, t);
       n = x.pieces(c);
     }
     const int cut = n > 1 ? x.rows * heads : 0;
     int v[4] = {n, n > 1, n * cut, cut}, total[4];
     scan(v, total, sh);
     const int e0 = n_entries + v[0], part = n_parts + v[2];
-    for (int i = 0; i < n && e0 + i < max_entries; ++i) {
+    for (int i = 0; i < n && e0 + i < to.max_entries; ++i) {
       const int lo = static_cast<int>(static_cast<int64_t>(x.kv) * i / n);
       const int hi = static_cast<int>(static_cast<int64_t>(x.kv) * (i + 1) / n);
-      entries[e0 + i] = {x.seq, x.row0, x.rows, lo, hi, n > 1 ? part + i * cut : -1, 0, 0};
+      to.entries[e0 + i] = {x.seq, x.row0, x.rows, lo, hi, n > 1 ? part + i * cut : -1, 0, 0};
     }
-    if (n > 1) splits[n_splits + v[1]] = {x.seq, x.row0, x.rows, n, part, n_rows + v[3], 0, 0};
+    if (n > 1) to.splits[n_splits + v[1]] = {x.seq, x.row0, x.rows, n, part, n_rows + v[3], 0, 0};
     n_entries += total[0];
     n_splits += total[1];
     n_parts += total[2];
     n_rows += total[3];
   }
-  if (tid == 0) *plan = {min(n_entries, max_entries), n_splits, n_rows, 0};
+  if (tid == 0) *to.plan = {min(n_entries, to.max_entries), n_splits, n_rows, 0};
 }
 
 // Merge of split rows, a warp per row: with M = max m_p and w_p = 2^(m_p - M),
 // o = sum w_p o_p / sum w_p l_p.  It moves a few MB; what it costs is the launch.
 constexpr int kMergeThreads = 256;
 template <int D>
-__global__ void __launch_bounds__(kMergeThreads) extend_merge_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kMergeThreads)
+extend_merge_kernel(const __grid_constant__ Params many, const __grid_constant__ Params few) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const ExtendArgs& a = p.a;
+  const ExtendArgs& a = many.a;
   const int lane = threadIdx.x & 31, heads = a.n_kv_heads;
   constexpr int E = D / 32;
-  const Plan plan = *p.plan;
-  for (int g = (blockIdx.x * kMergeThreads + threadIdx.x) >> 5; g < plan.split_rows;
-       g += gridDim.x * (kMergeThreads / 32)) {
-    int lo = 0, hi = plan.n_splits - 1;
+  const int n_many = many.plan->split_rows, n_all = n_many + few.plan->split_rows;
+  for (int i = (blockIdx.x * kMergeThreads + threadIdx.x) >> 5; i < n_all; i += gridDim.x * (kMergeThreads / 32)) {
+    const Params& p = i < n_many ? many : few;
+    const int g = i < n_many ? i : i - n_many;
+    int lo = 0, hi = p.plan->n_splits - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (p.splits[mid].first <= g) lo = mid; else hi = mid - 1;
@@ -265,16 +287,16 @@ bool plane_aligned(const Plane& p, int head_dim) {
   return rows(p.scales, p.ss) && (p.mode != KNLP_KV_INT4_ASYM || rows(p.zeros, p.zs));
 }
 
-int launch_modes(const Params& p, int grid, cudaStream_t st) {
+int launch_modes(const Params& p, const Params& few, int grid, cudaStream_t st) {
   const int k = p.a.k.mode == KNLP_KV_BF16 ? kRaw : p.a.k.mode, v = p.a.v.mode;
-  if (k == KNLP_KV_INT4_ASYM && v == KNLP_KV_INT4_ASYM) return launch_extend_pair<KNLP_KV_INT4_ASYM, KNLP_KV_INT4_ASYM>(p, grid, st);
-  if (k == KNLP_KV_INT4_SYM && v == KNLP_KV_INT4_SYM) return launch_extend_pair<KNLP_KV_INT4_SYM, KNLP_KV_INT4_SYM>(p, grid, st);
-  if (k == KNLP_KV_INT8_G32 && v == KNLP_KV_INT4_ASYM) return launch_extend_pair<KNLP_KV_INT8_G32, KNLP_KV_INT4_ASYM>(p, grid, st);
-  if (k == KNLP_KV_INT8_G32 && v == KNLP_KV_INT4_SYM) return launch_extend_pair<KNLP_KV_INT8_G32, KNLP_KV_INT4_SYM>(p, grid, st);
-  if (k == KNLP_KV_INT8_G32 && v == KNLP_KV_INT8_G32) return launch_extend_pair<KNLP_KV_INT8_G32, KNLP_KV_INT8_G32>(p, grid, st);
-  if (k == kRaw && v == KNLP_KV_INT4_ASYM) return launch_extend_pair<kRaw, KNLP_KV_INT4_ASYM>(p, grid, st);
-  if (k == kRaw && v == KNLP_KV_INT4_SYM) return launch_extend_pair<kRaw, KNLP_KV_INT4_SYM>(p, grid, st);
-  if (k == kRaw && v == KNLP_KV_INT8_G32) return launch_extend_pair<kRaw, KNLP_KV_INT8_G32>(p, grid, st);
+  if (k == KNLP_KV_INT4_ASYM && v == KNLP_KV_INT4_ASYM) return launch_extend_pair<KNLP_KV_INT4_ASYM, KNLP_KV_INT4_ASYM>(p, few, grid, st);
+  if (k == KNLP_KV_INT4_SYM && v == KNLP_KV_INT4_SYM) return launch_extend_pair<KNLP_KV_INT4_SYM, KNLP_KV_INT4_SYM>(p, few, grid, st);
+  if (k == KNLP_KV_INT8_G32 && v == KNLP_KV_INT4_ASYM) return launch_extend_pair<KNLP_KV_INT8_G32, KNLP_KV_INT4_ASYM>(p, few, grid, st);
+  if (k == KNLP_KV_INT8_G32 && v == KNLP_KV_INT4_SYM) return launch_extend_pair<KNLP_KV_INT8_G32, KNLP_KV_INT4_SYM>(p, few, grid, st);
+  if (k == KNLP_KV_INT8_G32 && v == KNLP_KV_INT8_G32) return launch_extend_pair<KNLP_KV_INT8_G32, KNLP_KV_INT8_G32>(p, few, grid, st);
+  if (k == kRaw && v == KNLP_KV_INT4_ASYM) return launch_extend_pair<kRaw, KNLP_KV_INT4_ASYM>(p, few, grid, st);
+  if (k == kRaw && v == KNLP_KV_INT4_SYM) return launch_extend_pair<kRaw, KNLP_KV_INT4_SYM>(p, few, grid, st);
+  if (k == kRaw && v == KNLP_KV_INT8_G32) return launch_extend_pair<kRaw, KNLP_KV_INT8_G32>(p, few, grid, st);
   return 1;
 }
 
@@ -283,19 +305,21 @@ bool pair_built(int k, int v) {
   return raw || k == KNLP_KV_INT8_G32 || k == v;
 }
 
-// Workspace, in ints / floats: plan, first tile of each sequence, pieces, splits, partial rows.
+// Workspace, in ints / floats, for each kernel: plan, first tile of each sequence, pieces, splits,
+// partial rows.
 struct Sizes {
-  int64_t entries, splits, parts, base_at, entries_at, splits_at, parts_at, floats;
-  Sizes(int n_seqs, int n_tokens, int n_q_heads, int n_kv_heads, int head_dim, int n_sms) {
-    const int64_t rows = static_cast<int64_t>(n_tokens) * (n_q_heads / n_kv_heads);
-    entries = entries_bound(n_seqs, rows, n_kv_heads, n_sms);
-    splits = tiles_bound(n_seqs, rows);
-    parts = parts_bound(n_tokens, n_q_heads, n_sms);
-    base_at = 4;
-    entries_at = (base_at + n_seqs + 1 + 3) / 4 * 4;
-    splits_at = entries_at + entries * 8;
-    parts_at = splits_at + splits * 8;
-    floats = parts_at + parts * (head_dim + 4) + 4;  // 4: alignment of the start
+  Bounds bounds[2];
+  int64_t at[2], entries_at[2], splits_at[2], parts_at[2], floats = 0;
+  Sizes(int n_seqs, int n_tokens, int n_q_heads, int n_kv_heads, int head_dim, int n_sms)
+      : bounds{{false, n_seqs, n_tokens, n_q_heads, n_kv_heads, n_sms}, {true, n_seqs, n_tokens, n_q_heads, n_kv_heads, n_sms}} {
+    for (int i = 0; i < 2; ++i) {
+      at[i] = floats;
+      entries_at[i] = at[i] + (4 + n_seqs + 1 + 3) / 4 * 4;
+      splits_at[i] = entries_at[i] + bounds[i].entries * 8;
+      parts_at[i] = splits_at[i] + bounds[i].tiles * 8;
+      floats = parts_at[i] + bounds[i].parts * (head_dim + 4);
+    }
+    floats += 4;  // alignment of the start
   }
 };
 
@@ -322,28 +346,32 @@ int launch_extend_mma(const ExtendArgs& a, float* ws, int64_t ws_floats, int n_s
   if (mis) ws += (16 - mis) / 4;
   const Sizes z(a.n_seqs, a.n_tokens, a.n_q_heads, a.n_kv_heads, a.head_dim, n_sms);
   if (ws_floats < z.floats) return KNLP_ERR_WORKSPACE;
-  Params p{};
-  p.a = a;
-  int* base = reinterpret_cast<int*>(ws + z.base_at);
-  Plan* plan = reinterpret_cast<Plan*>(ws);
-  Entry* entries = reinterpret_cast<Entry*>(ws + z.entries_at);
-  Split* splits = reinterpret_cast<Split*>(ws + z.splits_at);
-  p.plan = plan;
-  p.entries = entries;
-  p.splits = splits;
-  p.parts = ws + z.parts_at;
-  p.status = decode_status_ptr();
-  if (!p.status) return KNLP_ERR_NO_DEVICE;
-  p.rep = a.n_q_heads / a.n_kv_heads;
-  p.block_shift = -1;
-  for (int i = 0; i < 31; ++i)
-    if (a.block_size == 1 << i) p.block_shift = i;
-  extend_plan_kernel<<<1, kPlanThreads, 0, st>>>(a, p.rep, n_sms, static_cast<int>(z.entries),
-                                                 static_cast<int>(z.splits), z.parts, base, plan,
-                                                 entries, splits);
+  Params p[2]{};
+  Lists lists[2];
+  for (int i = 0; i < 2; ++i) {
+    Lists& l = lists[i];
+    l.max_entries = static_cast<int>(z.bounds[i].entries);
+    l.max_tiles = static_cast<int>(z.bounds[i].tiles);
+    l.max_parts = z.bounds[i].parts;
+    l.plan = reinterpret_cast<Plan*>(ws + z.at[i]);
+    l.base = reinterpret_cast<int*>(ws + z.at[i] + 4);
+    l.entries = reinterpret_cast<Entry*>(ws + z.entries_at[i]);
+    l.splits = reinterpret_cast<Split*>(ws + z.splits_at[i]);
+    p[i].a = a;
+    p[i].plan = l.plan;
+    p[i].entries = l.entries;
+    p[i].splits = l.splits;
+    p[i].parts = ws + z.parts_at[i];
+    p[i].status = decode_status_ptr();
+    if (!p[i].status) return KNLP_ERR_NO_DEVICE;
+    p[i].rep = a.n_q_heads / a.n_kv_heads;
+    p[i].block_shift = -1;
+    for (int b = 0; b < 31; ++b)
+      if (a.block_size == 1 << b) p[i].block_shift = b;
+  }
+  extend_plan_kernel<<<2, kPlanThreads, 0, st>>>(a, p[0].rep, n_sms, lists[0], lists[1]);
   if (cudaGetLastError() != cudaSuccess) return KNLP_ERR_LAUNCH;
-  const int64_t items = z.entries * a.n_kv_heads;
-  const int rc = launch_modes(p, static_cast<int>(items < n_sms ? items : n_sms), st);
+  const int rc = launch_modes(p[0], p[1], n_sms, st);
   if (rc != KNLP_OK) return rc > 0 ? KNLP_ERR_MODE : rc;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(2 * n_sms);
@@ -354,8 +382,8 @@ int launch_extend_mma(const ExtendArgs& a, float* ws, int64_t ws_floats, int n_s
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t err = a.head_dim == 64 ? cudaLaunchKernelEx(&cfg, extend_merge_kernel<64>, p)
-                                           : cudaLaunchKernelEx(&cfg, extend_merge_kernel<128>, p);
+  const cudaError_t err = a.head_dim == 64 ? cudaLaunchKernelEx(&cfg, extend_merge_kernel<64>, p[0], p[1])
+                                           : cudaLaunchKernelEx(&cfg, extend_merge_kernel<128>, p[0], p[1]);
   if (err != cudaSuccess) {
     cudaGetLastError();
     return KNLP_ERR_LAUNCH;
