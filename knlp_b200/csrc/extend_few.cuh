@@ -66,7 +66,7 @@ struct FewMisc {
   int abort;
   // per query row
   alignas(16) float off[kFewRows];  // -m, the reference of its exponents; read as float4
-  float delta[kFewRows];  // what a rescaling adds to m
+  float delta[kFewRows], factor[kFewRows];  // what a rescaling adds to m, 2^-delta
   float most[4][kFewRows];  // maxima of the warps
   int limit[kFewRows];      // cached tokens that it attends to
   int64_t out_row[kFewRows];
@@ -106,15 +106,16 @@ __device__ __forceinline__ bool any_of_128(bool x) {
 }
 __device__ __forceinline__ void sync_128() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
-// Every other tile of a plane, counted over all items, by one warpgroup into its own slot.
-template <class L, int MODE, int D, int SIDE, int PHASE>
-__device__ __forceinline__ void few_produce(const Params& p, char* sm, FewMisc& mi, int n_items, int w, int lane) {
+// Every other tile of a plane, counted over all items, by one warpgroup into its own slot.  The
+// warpgroups of a plane, and planes of one mode, run the same code (see produce).
+template <class L, int MODE, int D, int STAGES>
+__device__ __forceinline__ void few_produce(const Params& p, char* sm, FewMisc& mi, int n_items, int side, int phase, int w, int lane) {
   using T = PlaneTile<MODE, D>;
-  constexpr int kStages = SIDE ? L::kStagesV : L::kStagesK;
-  char* const stages = sm + (SIDE ? L::kStageV : L::kStageK) + PHASE * kStages * T::kBytes;
-  char* const to = sm + L::kKV + (SIDE * 2 + PHASE) * L::kTileBytes;
+  constexpr int kStages = STAGES;
+  char* const stages = sm + (side ? L::kStageV : L::kStageK) + phase * kStages * T::kBytes;
+  char* const to = sm + L::kKV + (side * 2 + phase) * L::kTileBytes;
   const int row = w * 32 + lane;
-  Copies<MODE, D, SIDE, PHASE> copies(p, n_items, w, lane);
+  Copies<MODE, D, 2> copies(p, side ? p.a.v : p.a.k, n_items, w, lane, phase);
   for (int i = 0; i < kStages; ++i) copies.next(stages + i * T::kBytes);
   uint32_t count = 0, use = 0, stage = 0;
   int serial = 0;
@@ -123,28 +124,28 @@ __device__ __forceinline__ void few_produce(const Params& p, char* sm, FewMisc& 
     const int n = it.tiles();
     if (n == 0) continue;
     BadList& bad = mi.bad[serial % kBadLists];
-    if constexpr (SIDE == 1) {
-      if (PHASE == 0 && row == 0) bad.clear();
+    if (side) {
+      if (phase == 0 && row == 0) bad.clear();
       asm volatile("bar.sync 3, 256;" ::: "memory");  // both warpgroups of V
     }
-    for (int j = (count & 1) != PHASE; j < n; j += 2, ++use) {
+    for (int j = (count & 1) != phase; j < n; j += 2, ++use) {
       if constexpr (kStages == 0) {
-        mbar_wait(&mi.empty[SIDE][PHASE], (use + 1) & 1, &mi.abort, p.status);
+        mbar_wait(&mi.empty[side][phase], (use + 1) & 1, &mi.abort, p.status);
         copies.next(to);
         asm volatile("cp.async.wait_group 0;" ::: "memory");
       } else {
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
         __syncwarp();
         char* const from = stages + stage * T::kBytes;
-        if constexpr (SIDE == 1) {
-          if (any_not_finite<MODE, D>(from, row)) bad.note<MODE, D>(from, row, (it.e.tile0 + j) * kTile + row);
+        if constexpr (T::kQuant) {
+          if (side && any_not_finite<MODE, D>(from, row)) bad.note<MODE, D>(from, row, (it.e.tile0 + j) * kTile + row);
         }
-        mbar_wait(&mi.empty[SIDE][PHASE], (use + 1) & 1, &mi.abort, p.status);
+        mbar_wait(&mi.empty[side][phase], (use + 1) & 1, &mi.abort, p.status);
         dequantize_row<MODE, D>(from, to, row);
       }
       fence_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&mi.full[SIDE][PHASE]);
+      if (lane == 0) mbar_arrive(&mi.full[side][phase]);
       if constexpr (kStages > 0) {
         copies.next(stages + stage * T::kBytes);
         stage = stage + 1 == kStages ? 0 : stage + 1;
@@ -279,6 +280,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) extend_few_kernel(const __grid
             if (tid < rows) v = fmaxf(fmaxf(mi.most[0][tid], mi.most[1][tid]), fmaxf(mi.most[2][tid], mi.most[3][tid]));
             const float by = j == 0 ? (v == -INFINITY ? 0.0f : v) : fmaxf(v, 0.0f);
             mi.delta[tid] = by;
+            mi.factor[tid] = exp2f(-by);
             mi.off[tid] -= by;
           }
           sync_128();
@@ -293,7 +295,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) extend_few_kernel(const __grid
                 tmem_ld16(tmem + lanes + acc + x0, o);
                 tmem_wait_ld16(o);
 #pragma unroll
-                for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * exp2f(-mi.delta[x0 + x]));
+                for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * mi.factor[x0 + x]);
                 tmem_st16(tmem + lanes + acc + x0, o);
               }
             }
@@ -327,7 +329,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) extend_few_kernel(const __grid
         if (lane == 0) mbar_arrive(&mi.p_full);
       }
 
-      // a thread per column of O as the accumulator has it, 16 rows at a time
+      // a thread per column of O as the accumulator has it, 4 rows at a time
       if (n) {
         wait(&mi.o_full, n_o);
         fence_after();
@@ -338,19 +340,19 @@ __global__ void __launch_bounds__(kFewThreads, 1) extend_few_kernel(const __grid
       const bool direct = it.e.part < 0;
       float* part = p.parts + (static_cast<int64_t>(it.e.part) + static_cast<int64_t>(it.head) * rows) * (D + 4);
 #pragma unroll 1
-      for (int x0 = 0; x0 < rows; x0 += 16) {
-        uint32_t ou[16], lu[16];
+      for (int x0 = 0; x0 < rows; x0 += 4) {
+        uint32_t ou[4], lu[4];
         if (n) {
-          tmem_ld16(tmem + lanes + kTmemO + x0, ou);
-          tmem_ld16(tmem + lanes + kTmemL + x0, lu);
-          tmem_wait_ld16(ou);
-          tmem_wait_ld16(lu);
+          tmem_ld4(tmem + lanes + kTmemO + x0, ou);
+          tmem_ld4(tmem + lanes + kTmemL + x0, lu);
+          tmem_wait_ld4(ou);
+          tmem_wait_ld4(lu);
         } else {
 #pragma unroll
-          for (int x = 0; x < 16; ++x) ou[x] = lu[x] = 0;
+          for (int x = 0; x < 4; ++x) ou[x] = lu[x] = 0;
         }
 #pragma unroll
-        for (int x = 0; x < 16; ++x) {
+        for (int x = 0; x < 4; ++x) {
           const int r = x0 + x;
           if (r >= rows) break;
           const float l = __uint_as_float(lu[x]);
@@ -370,14 +372,14 @@ __global__ void __launch_bounds__(kFewThreads, 1) extend_few_kernel(const __grid
       fence_before();
       n_o += n > 0;
     }
-  } else if (warp < 8) {
-    few_produce<L, KM, D, 0, 0>(p, sm, mi, n_items, warp - 4, lane);
-  } else if (warp < 12) {
-    few_produce<L, KM, D, 0, 1>(p, sm, mi, n_items, warp - 8, lane);
-  } else if (warp < 16) {
-    few_produce<L, VM, D, 1, 0>(p, sm, mi, n_items, warp - 12, lane);
   } else if (warp < 20) {
-    few_produce<L, VM, D, 1, 1>(p, sm, mi, n_items, warp - 16, lane);
+    const int wg = (warp - 4) >> 2;  // K, K, V, V
+    if constexpr (KM == VM && L::kStagesK == L::kStagesV) {
+      few_produce<L, KM, D, L::kStagesK>(p, sm, mi, n_items, wg >> 1, wg & 1, warp & 3, lane);
+    } else {
+      if (wg < 2) few_produce<L, KM, D, L::kStagesK>(p, sm, mi, n_items, 0, wg, warp & 3, lane);
+      else few_produce<L, VM, D, L::kStagesV>(p, sm, mi, n_items, 1, wg - 2, warp & 3, lane);
+    }
   } else if (warp < 22) {
     // ---------------------------------------------------------------- matrix products
     auto wait_warp = [&](uint64_t* x, uint32_t phase) { mbar_wait_warp(x, phase & 1, &mi.abort, p.status); };

@@ -285,6 +285,13 @@ __device__ __forceinline__ void tmem_wait_ld16(uint32_t* r) {
         "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
       :: "memory");
 }
+__device__ __forceinline__ void tmem_ld4(uint32_t addr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld4(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]) :: "memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -356,10 +363,11 @@ __device__ __forceinline__ void dequantize_row(const char* stage, char* tile, in
     auto pick = [](const __half2* v, int g) { return g & 1 ? __high2half2(v[g >> 1]) : __low2half2(v[g >> 1]); };
 #pragma unroll
     for (int c = 0; c < P::kChunks; ++c) {
+      const int g = MODE == KNLP_KV_INT8_G32 ? c >> 1 : c;
       const uint4 w = *reinterpret_cast<const uint4*>(stage + P::at(row, c));
+      const __half2 sc = pick(s, g);
       const uint32_t u[4] = {w.x, w.y, w.z, w.w};
       if constexpr (MODE == KNLP_KV_INT8_G32) {  // 16 codes, half a group
-        const __half2 sc = pick(s, c >> 1);
         const __half2 bias = as_half2(0xe480e480u);  // -1152: the codes are biased by 128
         uint32_t o[8];
 #pragma unroll
@@ -371,9 +379,8 @@ __device__ __forceinline__ void dequantize_row(const char* stage, char* tile, in
         put(2 * c, make_uint4(o[0], o[1], o[2], o[3]));
         put(2 * c + 1, make_uint4(o[4], o[5], o[6], o[7]));
       } else {  // 32 codes, one group
-        const __half2 sc = pick(s, c);
         __half2 zc;
-        if constexpr (MODE == KNLP_KV_INT4_ASYM) zc = pick(z, c);
+        if constexpr (MODE == KNLP_KV_INT4_ASYM) zc = pick(z, g);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           __half2 h[4];
@@ -462,14 +469,14 @@ struct Item {
 };
 
 // Copies of one plane's tiles by a warpgroup, item after item: warp w copies rows 32 w .. 32 w + 31
-// of every tile, a lane looks up one row's block, a tile before it is needed.  PHASE >= 0: only
-// every other tile, counted over all items.
-template <int MODE, int D, int SIDE, int PHASE>
+// of every tile, a lane looks up one row's block, a tile before it is needed.  EVERY 2: only the
+// tiles of the parity `phase`, counted over all items.
+template <int MODE, int D, int EVERY>
 struct Copies {
   using T = PlaneTile<MODE, D>;
   const Params& p;
   const Plane& pl;
-  const int n_items, w, lane;
+  const int n_items, w, lane, phase;
   int k = blockIdx.x, tile = 0, tile1 = 0, len = 0, block = 0, off = 0;
   uint32_t count = 0;  // tiles of the items so far
   const int32_t* table = nullptr;
@@ -477,16 +484,16 @@ struct Copies {
   int64_t head_scales = 0, head_zeros = 0;
   bool there = false, pending;  // pending: a tile is looked up
 
-  __device__ __forceinline__ Copies(const Params& p_, int n_items_, int w_, int lane_)
-      : p(p_), pl(SIDE ? p_.a.v : p_.a.k), n_items(n_items_), w(w_), lane(lane_) {
+  __device__ __forceinline__ Copies(const Params& p_, const Plane& plane, int n_items_, int w_, int lane_, int phase_)
+      : p(p_), pl(plane), n_items(n_items_), w(w_), lane(lane_), phase(phase_) {
     pending = look_up();
   }
   __device__ __forceinline__ bool look_up() {
     while (tile >= tile1 && k < n_items) {  // the first tile of the next item that has any
       const Item it(p, k);
       tile = it.e.tile0, tile1 = it.e.tile1, len = it.len;
-      if constexpr (PHASE >= 0) {
-        tile += (count & 1) != PHASE;
+      if constexpr (EVERY == 2) {
+        tile += (count & 1) != phase;
         count += it.tiles();
       }
       table = p.a.block_table + it.e.seq * p.a.bt_stride;
@@ -503,7 +510,7 @@ struct Copies {
     const int e = p.block_shift >= 0 ? t >> p.block_shift : t / p.a.block_size;
     off = t - e * p.a.block_size;
     block = there ? table[e] : 0;
-    tile += PHASE >= 0 ? 2 : 1;
+    tile += EVERY;
     return true;
   }
   // The looked-up tile to `dst`, a stage (or the operand itself, unquantized), as one group of
@@ -589,29 +596,30 @@ struct Misc {
 };
 static_assert(sizeof(Misc) <= kMiscBytes, "");
 
-// One plane's tiles (SIDE 0: K, 1: V) by a warpgroup: a lane converts one row of every tile, and
-// only lanes of the same warp read what a lane has copied.
-template <class L, int MODE, int D, int SIDE>
-__device__ __forceinline__ void produce(const Params& p, char* sm, Misc& mi, int n_items, int w,
-                                        int lane) {
+// One plane's tiles (side 0: K, 1: V) by a warpgroup: a lane converts one row of every tile, and
+// only lanes of the same warp read what a lane has copied.  Planes of one mode run the same code:
+// the instruction cache is what several warpgroups of unrolled code compete for.
+template <class L, int MODE, int D, int STAGES>
+__device__ __forceinline__ void produce(const Params& p, char* sm, Misc& mi, int n_items, int side,
+                                        int w, int lane) {
   using T = PlaneTile<MODE, D>;
-  constexpr int kStages = SIDE ? L::kStagesV : L::kStagesK;
-  char* const stages = sm + (SIDE ? L::kStageV : L::kStageK);
+  constexpr int kStages = STAGES;
+  char* const stages = sm + (side ? L::kStageV : L::kStageK);
   const int row = w * 32 + lane;
-  Copies<MODE, D, SIDE, -1> copies(p, n_items, w, lane);
+  Copies<MODE, D, 1> copies(p, side ? p.a.v : p.a.k, n_items, w, lane, 0);
   for (int i = 0; i < kStages; ++i) copies.next(stages + i * T::kBytes);
-  uint32_t done = SIDE, stage = 0;  // done: number of the plane tile in the ring's order
+  uint32_t done = side, stage = 0;  // done: number of the plane tile in the ring's order
   // The slot's use before this one, always the other plane's, has to be over.
   auto wait_empty = [&]() {
     const uint32_t others = (done / kRing + 1) / 2;  // uses of this slot by the other plane
-    mbar_wait(&mi.ring_empty[1 - SIDE][done % kRing], (others + 1) & 1, &mi.abort, p.status);
+    mbar_wait(&mi.ring_empty[1 - side][done % kRing], (others + 1) & 1, &mi.abort, p.status);
   };
   int serial = 0;
   for (int ki = blockIdx.x; ki < n_items; ki += gridDim.x) {
     const Item it(p, ki);
     if (it.tiles() == 0) continue;
     BadList& bad = mi.bad[serial % kBadLists];
-    if constexpr (SIDE == 1) {
+    if (side) {
       if (row == 0) bad.clear();
       asm volatile("bar.sync 3, 128;" ::: "memory");
     }
@@ -625,8 +633,8 @@ __device__ __forceinline__ void produce(const Params& p, char* sm, Misc& mi, int
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
         __syncwarp();
         char* const from = stages + stage * T::kBytes;
-        if constexpr (SIDE == 1) {
-          if (any_not_finite<MODE, D>(from, row)) bad.note<MODE, D>(from, row, (it.e.tile0 + j) * kTile + row);
+        if constexpr (T::kQuant) {
+          if (side && any_not_finite<MODE, D>(from, row)) bad.note<MODE, D>(from, row, (it.e.tile0 + j) * kTile + row);
         }
         wait_empty();
         dequantize_row<MODE, D>(from, to, row);
@@ -719,7 +727,7 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
         constexpr int kPer = D / 8, kAtOnce = 32 / kPer;
         char* q = sm + L::kQ + w * L::kTileBytes;
         const int r0 = (warp & 3) * 32, chunk = lane % kPer;
-#pragma unroll 4
+#pragma unroll 2
         for (int i = 0; i < 32; i += kAtOnce) {
           const int r = r0 + i + lane / kPer;
           const int lr = (it.pair() ? w * kRows : 0) + r;
@@ -831,7 +839,7 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
       const bool merge = !it.pair() && steps > 0;
       if (merge && w == 1) {
         if (active) {
-#pragma unroll
+#pragma unroll 1  // run once per item: straight-line code would come from memory, not from the cache
           for (int i = 0; i < D; i += 32) {
             uint32_t o[32];
             tmem_ld32(t_o + i, o);
@@ -861,7 +869,7 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
         const int64_t out_row = (static_cast<int64_t>(it.first) + tok) * a.n_q_heads + it.head * p.rep + h;
         float* part = direct ? nullptr
                              : p.parts + (static_cast<int64_t>(it.e.part) + static_cast<int64_t>(it.head) * it.e.rows + local) * (D + 4);
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < D; i += 32) {
           float o[32];
           if (steps) {
@@ -927,8 +935,12 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
     }
   } else if (warp < 16) {
     KNLP_REGISTERS("dec", 80);
-    if (warp < 12) produce<L, KM, D, 0>(p, sm, mi, n_items, warp - 8, lane);
-    else produce<L, VM, D, 1>(p, sm, mi, n_items, warp - 12, lane);
+    if constexpr (KM == VM && L::kStagesK == L::kStagesV) {
+      produce<L, KM, D, L::kStagesK>(p, sm, mi, n_items, (warp - 8) >> 2, warp & 3, lane);
+    } else {
+      if (warp < 12) produce<L, KM, D, L::kStagesK>(p, sm, mi, n_items, 0, warp & 3, lane);
+      else produce<L, VM, D, L::kStagesV>(p, sm, mi, n_items, 1, warp & 3, lane);
+    }
   } else {
     // ---------------------------------------------------------------- matrix products
     KNLP_REGISTERS("dec", 48);
