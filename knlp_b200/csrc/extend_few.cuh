@@ -218,7 +218,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) extend_few_kernel(const __grid
       }
       if (n) {
         constexpr int kPer = D / 8;  // 16-byte chunks of a row
-        for (int i = tid; i < kFewRows * kPer; i += 128) {
+#pragma unroll
+        for (int i0 = 0; i0 < kFewRows * kPer; i0 += 128) {
+          const int i = i0 + tid;
           const int r = i / kPer, chunk = i % kPer;
           uint4 v = make_uint4(0, 0, 0, 0);
           if (r < rows) {

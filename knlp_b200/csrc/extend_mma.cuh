@@ -723,23 +723,33 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
 
       asm volatile("bar.sync 1, 256;" ::: "memory");  // nobody reads the Q area any more
       if (it.tiles() && (w == 0 || it.pair())) {
-        // Q tile: D/8 lanes copy a row, 16 bytes each
+        // Q tile: D/8 lanes copy a row, 16 bytes each; a lane works out the place of one row, and
+        // eight loads are in flight
         constexpr int kPer = D / 8, kAtOnce = 32 / kPer;
         char* q = sm + L::kQ + w * L::kTileBytes;
         const int r0 = (warp & 3) * 32, chunk = lane % kPer;
-#pragma unroll 2
-        for (int i = 0; i < 32; i += kAtOnce) {
-          const int r = r0 + i + lane / kPer;
-          const int lr = (it.pair() ? w * kRows : 0) + r;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (lr < it.e.rows) {
-            const int f = it.e.row0 + lr, t = f / p.rep;
-            const int64_t off = (static_cast<int64_t>(it.first) + t) * a.q_stride[0] +
-                                (static_cast<int64_t>(it.head) * p.rep + (f - t * p.rep)) * a.q_stride[1];
-            v = reinterpret_cast<const uint4*>(static_cast<const char*>(a.q) + 2 * off)[chunk];
+        const int f = rw.flat, t = rw.tok;
+        const char* mine = nullptr;
+        if (rw.valid)
+          mine = static_cast<const char*>(a.q) + 2 * ((static_cast<int64_t>(it.first) + t) * a.q_stride[0] +
+                                                      (static_cast<int64_t>(it.head) * p.rep + (f - t * p.rep)) * a.q_stride[1]);
+        const uint32_t lo = static_cast<uint32_t>(reinterpret_cast<uint64_t>(mine));
+        const uint32_t hi = static_cast<uint32_t>(reinterpret_cast<uint64_t>(mine) >> 32);
+#pragma unroll 1
+        for (int i0 = 0; i0 < 32; i0 += 8 * kAtOnce) {
+          uint4 v[8];
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const int r = i0 + x * kAtOnce + lane / kPer;
+            const uint64_t from = static_cast<uint64_t>(__shfl_sync(~0u, hi, r)) << 32 | __shfl_sync(~0u, lo, r);
+            v[x] = from ? reinterpret_cast<const uint4*>(from)[chunk] : make_uint4(0, 0, 0, 0);
           }
-          *reinterpret_cast<uint4*>(q + (chunk >> 3) * (kRows * 128) + r * 128 +
-                                    (((chunk & 7) ^ (r & 7)) << 4)) = query_operand<KM>(v, a.q_dtype);
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const int r = r0 + i0 + x * kAtOnce + lane / kPer;
+            *reinterpret_cast<uint4*>(q + (chunk >> 3) * (kRows * 128) + r * 128 +
+                                      (((chunk & 7) ^ (r & 7)) << 4)) = query_operand<KM>(v[x], a.q_dtype);
+          }
         }
         fence_smem();
       }
