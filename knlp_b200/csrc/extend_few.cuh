@@ -119,7 +119,7 @@ __device__ __forceinline__ void few_produce(const Params& p, char* sm, FewMisc& 
   for (int i = 0; i < kStages; ++i) copies.next(stages + i * T::kBytes);
   uint32_t count = 0, use = 0, stage = 0;
   int serial = 0;
-  for (int ki = blockIdx.x; ki < n_items; ki += gridDim.x) {
+  for (int r = 0, ki; (ki = item_of(r)) < n_items; ++r) {
     const Item it(p, ki);
     const int n = it.tiles();
     if (n == 0) continue;
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) extend_few_kernel(const __grid
     // ---------------------------------------------------------------- softmax and results
     const float c = a.scale * kLog2e;
     uint32_t count = 0, n_o = 0;  // tiles, items with tiles so far
-    for (int k = blockIdx.x; k < n_items; k += gridDim.x) {
+    for (int r = 0, k; (k = item_of(r)) < n_items; ++r) {
       const Item it(p, k);
       const int rows = it.e.rows, n = it.tiles();
       sync_128();  // the last item's tables and query are not in use any more
@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) extend_few_kernel(const __grid
     const uint32_t tm = uniform(tmem);
     const int n_all = uniform(n_items);
     uint32_t count = 0, n_q = 0;
-    for (int k = blockIdx.x; k < n_all; k += gridDim.x) {
+    for (int r = 0, k; (k = item_of(r)) < n_all; ++r) {
       const Item it(p, k);
       const int n = uniform(it.tiles());
       if (n == 0) continue;

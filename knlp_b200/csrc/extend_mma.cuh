@@ -448,6 +448,13 @@ __device__ __forceinline__ uint4 query_operand(uint4 v, int dtype) {
   return v;
 }
 
+// A CTA's item of a round.  The list is sorted by length, longest first, and dealt out back and
+// forth, so that a CTA's sum is even.
+__device__ __forceinline__ int item_of(int r) {
+  const int g = gridDim.x, b = blockIdx.x;
+  return r * g + (r & 1 ? g - 1 - b : b);
+}
+
 // Geometry of an item that every role derives for itself.
 struct Item {
   Entry e;
@@ -477,7 +484,7 @@ struct Copies {
   const Params& p;
   const Plane& pl;
   const int n_items, w, lane, phase;
-  int k = blockIdx.x, tile = 0, tile1 = 0, len = 0, block = 0, off = 0;
+  int round = 0, tile = 0, tile1 = 0, len = 0, block = 0, off = 0;
   uint32_t count = 0;  // tiles of the items so far
   const int32_t* table = nullptr;
   const char* head_codes = nullptr;
@@ -489,7 +496,7 @@ struct Copies {
     pending = look_up();
   }
   __device__ __forceinline__ bool look_up() {
-    while (tile >= tile1 && k < n_items) {  // the first tile of the next item that has any
+    for (int k; tile >= tile1 && (k = item_of(round)) < n_items; ++round) {  // the first tile of the next item that has any
       const Item it(p, k);
       tile = it.e.tile0, tile1 = it.e.tile1, len = it.len;
       if constexpr (EVERY == 2) {
@@ -502,7 +509,6 @@ struct Copies {
         head_scales = it.head * pl.ss[2];
         head_zeros = it.head * pl.zs[2];
       }
-      k += gridDim.x;
     }
     if (tile >= tile1) return false;
     const int t = tile * kTile + w * 32 + lane;
@@ -615,7 +621,7 @@ __device__ __forceinline__ void produce(const Params& p, char* sm, Misc& mi, int
     mbar_wait(&mi.ring_empty[1 - side][done % kRing], (others + 1) & 1, &mi.abort, p.status);
   };
   int serial = 0;
-  for (int ki = blockIdx.x; ki < n_items; ki += gridDim.x) {
+  for (int r = 0, ki; (ki = item_of(r)) < n_items; ++r) {
     const Item it(p, ki);
     if (it.tiles() == 0) continue;
     BadList& bad = mi.bad[serial % kBadLists];
@@ -711,7 +717,7 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
         limit = !valid ? 0 : p.a.causal ? max(min(it.ctx + tok + 1, it.len), 0) : it.len;
       }
     };
-    for (int k = blockIdx.x; k < n_items; k += gridDim.x) {
+    for (int r = 0, k; (k = item_of(r)) < n_items; ++r) {
       float m = -INFINITY, l = 0.0f;
       {
       const Item it(p, k);
@@ -1004,7 +1010,7 @@ __global__ void __launch_bounds__(kThreads, 1) extend_mma_kernel(const __grid_co
         fence_after();
         return x % kRing;
       };
-      for (int k = blockIdx.x; k < n_all; k += gridDim.x) {
+      for (int r = 0, k; (k = item_of(r)) < n_all; ++r) {
         const Item it(p, k);
         const int n = uniform(it.tiles());
         if (n == 0) continue;

@@ -118,7 +118,8 @@ extend_plan_kernel(const __grid_constant__ ExtendArgs a, int rep, int n_ctas, co
   const Lists& to = few_rows ? few : many;
   int* const base = to.base;
   __shared__ int sh[4][kPlanThreads / 32];
-  __shared__ float sh_cost[kCandidates], sh_piece[kCandidates];
+  __shared__ float sh_cost[kCandidates], sh_piece[kCandidates], sh_worst[kCandidates];
+  __shared__ int sh_at[kPlanThreads];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int heads = a.n_kv_heads;
 
@@ -177,12 +178,31 @@ extend_plan_kernel(const __grid_constant__ ExtendArgs a, int rep, int n_ctas, co
     if (warp == 0) est = fminf(est, 1e29f);  // always possible
     sh_cost[warp] = est;
     sh_piece[warp] = piece;
+    sh_worst[warp] = worst;
   }
   __syncthreads();
   int best = 0;
   for (int w = 1; w < kCandidates; ++w)
     if (sh_cost[w] < sh_cost[best]) best = w;
   const float c = sh_piece[best];
+
+  // Where the pieces of each length begin, longest first, by counting: kPlanThreads classes.
+  const float per_class = (kPlanThreads - 1) / fmaxf(sh_worst[best], 1.0f);
+  auto class_of = [&](const Tile& x, int n) {
+    return kPlanThreads - 1 - min(kPlanThreads - 1, static_cast<int>(x.cost() / n * per_class));
+  };
+  sh_at[tid] = 0;
+  __syncthreads();
+  for (int t = tid; t < n_tiles; t += kPlanThreads) {
+    const Tile x = tile_at(a, few_rows, rep, base, t);
+    const int n = x.pieces(c);
+    atomicAdd(&sh_at[class_of(x, n)], n);
+  }
+  __syncthreads();
+  int first[1] = {sh_at[tid]}, all[1];
+  scan(first, all, sh);
+  sh_at[tid] = first[0];
+  __syncthreads();
 
   int n_entries = 0, n_splits = 0, n_parts = 0, n_rows = 0;
   for (int t0 = 0; t0 < n_tiles; t0 += kPlanThreads) {
@@ -196,7 +216,7 @@ extend_plan_kernel(const __grid_constant__ ExtendArgs a, int rep, int n_ctas, co
     const int cut = n > 1 ? x.rows * heads : 0;
     int v[4] = {n, n > 1, n * cut, cut}, total[4];
     scan(v, total, sh);
-    const int e0 = n_entries + v[0], part = n_parts + v[2];
+    const int e0 = n ? atomicAdd(&sh_at[class_of(x, n)], n) : 0, part = n_parts + v[2];
     for (int i = 0; i < n && e0 + i < to.max_entries; ++i) {
       const int lo = static_cast<int>(static_cast<int64_t>(x.kv) * i / n);
       const int hi = static_cast<int>(static_cast<int64_t>(x.kv) * (i + 1) / n);
