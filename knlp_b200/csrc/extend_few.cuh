@@ -8,12 +8,14 @@
 // tokens is 20 KB, 890 cycles at the SM's share of the measured bandwidth, and 32 K values).  With
 // rows on M, as the kernel for many rows has them, 3/4 of the products and of the softmax lanes
 // would serve nothing, on two of the eight softmax warps; here a tile's products take 3 x 320
-// tensor cycles at N = 32 and all four softmax warps share its exponentials.
+// tensor cycles at N = 32 and all eight softmax warps share its exponentials.
 //
-// One CTA per SM, 24 warps of at most 80 registers:
-//   warps 0-3    softmax, a thread per token of the tile, and the result (a thread per column of O)
-//   warps 4-19   dequantization: two warpgroups for K, two for V, every other tile each
-//   warp 20, 21  issue the scores (four buffers, ahead of the softmax), the outputs
+// One CTA per SM, 28 warps of at most 72 registers:
+//   warps 0-3, 4-7  softmax, a thread per token of the tile; the second warpgroup has the upper
+//                   half of the rows (in groups of eight).  Then the result, a thread per column
+//                   of O, the rows dealt out to both
+//   warps 8-23      dequantization: two warpgroups for K, two for V, every other tile each
+//   warps 24, 25    issue the scores (four buffers, ahead of the softmax), the outputs
 // Two operand slots per plane, each filled by its own warpgroup.  P^T goes through shared memory
 // (64 bytes per token, 64-byte swizzle).
 //
@@ -29,7 +31,7 @@ namespace extend {
 namespace few {
 
 constexpr int kFewRows = 32;
-constexpr int kFewThreads = 24 * 32;
+constexpr int kFewThreads = 28 * 32;
 constexpr int kScoreBuffers = 4;
 
 // TMEM columns: four buffers of S^T, O^T, l, and a tile of ones (fp16 pairs) as an operand.
@@ -98,13 +100,15 @@ __device__ __forceinline__ void mma_ts2(uint32_t d, uint32_t a, uint32_t b, uint
 }
 constexpr uint32_t kAisMn = 1u << 15;  // instruction descriptor: A is MN-major
 
-__device__ __forceinline__ bool any_of_128(bool x) {
+// Of a warpgroup of the softmax, and of both.
+__device__ __forceinline__ bool any_of_128(int id, bool x) {
   uint32_t r;
-  asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbarrier.cta.red.or.pred q, 1, 128, p;\nselp.u32 %0, 1, 0, q;\n}"
-               : "=r"(r) : "r"(static_cast<uint32_t>(x)) : "memory");
+  asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbarrier.cta.red.or.pred q, %2, 128, p;\nselp.u32 %0, 1, 0, q;\n}"
+               : "=r"(r) : "r"(static_cast<uint32_t>(x)), "r"(id) : "memory");
   return r;
 }
-__device__ __forceinline__ void sync_128() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void sync_128(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ void sync_256() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 // Every other tile of a plane, counted over all items, by one warpgroup into its own slot.  The
 // warpgroups of a plane, and planes of one mode, run the same code (see produce).
@@ -169,16 +173,16 @@ __global__ void __launch_bounds__(kFewThreads, 1) extend_few_kernel(const __grid
   if (tid == 0) {
     for (int s = 0; s < 2; ++s)
       for (int i = 0; i < 2; ++i) mbar_init(&mi.full[s][i], 4), mbar_init(&mi.empty[s][i], 1);
-    for (int i = 0; i < kScoreBuffers; ++i) mbar_init(&mi.s_full[i], 1), mbar_init(&mi.s_free[i], 4);
-    mbar_init(&mi.q_full, 4);
-    mbar_init(&mi.p_full, 4);
+    for (int i = 0; i < kScoreBuffers; ++i) mbar_init(&mi.s_full[i], 1), mbar_init(&mi.s_free[i], 8);
+    mbar_init(&mi.q_full, 8);
+    mbar_init(&mi.p_full, 8);
     mbar_init(&mi.p_free, 1);
     mbar_init(&mi.o_full, 1);
     mi.abort = 0;
     for (int i = 0; i < kBadLists; ++i) mi.bad[i].clear();
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 20) {
+  if (warp == 24) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&mi.tmem)), "n"(kTmemColumns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -202,14 +206,15 @@ __global__ void __launch_bounds__(kFewThreads, 1) extend_few_kernel(const __grid
   const int n_items = p.plan->n_entries * a.n_kv_heads;
   auto wait = [&](uint64_t* b, uint32_t phase) { mbar_wait(b, phase & 1, &mi.abort, p.status); };
 
-  if (warp < 4) {
+  if (warp < 8) {
     // ---------------------------------------------------------------- softmax and results
     const float c = a.scale * kLog2e;
+    const int wg = warp >> 2, tok128 = tid & 127, bar = 4 + wg;
     uint32_t count = 0, n_o = 0;  // tiles, items with tiles so far
     for (int r = 0, k; (k = item_of(r)) < n_items; ++r) {
       const Item it(p, k);
       const int rows = it.e.rows, n = it.tiles();
-      sync_128();  // the last item's tables and query are not in use any more
+      sync_256();  // the last item's tables and query are not in use any more
       if (tid < kFewRows) {
         const int flat = it.e.row0 + tid, tok = flat / p.rep;
         mi.limit[tid] = tid >= rows ? 0 : a.causal ? max(min(it.ctx + tok + 1, it.len), 0) : it.len;
@@ -219,9 +224,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) extend_few_kernel(const __grid
       if (n) {
         constexpr int kPer = D / 8;  // 16-byte chunks of a row
 #pragma unroll
-        for (int i0 = 0; i0 < kFewRows * kPer; i0 += 128) {
-          const int i = i0 + tid;
-          const int r = i / kPer, chunk = i % kPer;
+        for (int i0 = 0; i0 < kFewRows * kPer; i0 += 256) {
+          const int i = i0 + tid, r = i / kPer, chunk = i % kPer;
           uint4 v = make_uint4(0, 0, 0, 0);
           if (r < rows) {
             const int f = it.e.row0 + r, t = f / p.rep;
@@ -234,95 +238,103 @@ __global__ void __launch_bounds__(kFewThreads, 1) extend_few_kernel(const __grid
         }
         fence_smem();
       }
-      sync_128();
+      sync_256();
       if (n && lane == 0) mbar_arrive(&mi.q_full);
       // the fewest tokens that a row attends to: tiles below it need no mask
       const int least = __reduce_min_sync(~0u, lane < rows ? mi.limit[lane] : 0x7fffffff);
-      const int groups = (rows + 7) / 8;
+      // this warpgroup's rows: `mine` from `from` on, in groups of eight
+      const int groups = (rows + 7) / 8, lower = (groups + 1) / 2;
+      const int from = wg * lower * 8, mine = wg ? groups - lower : lower;
+      const int held = min(rows - from, mine * 8);
 
       for (int j = 0; j < n; ++j, ++count) {
-        const int token = (it.e.tile0 + j) * kTile + tid;
+        constexpr int kMine = kFewRows / 2;
+        const int token = (it.e.tile0 + j) * kTile + tok128;
         const uint32_t b = count % kScoreBuffers;
         wait(&mi.s_full[b], count / kScoreBuffers);
         fence_after();
-        float s[kFewRows];
-        tmem_ld32(tmem + lanes + b * kFewRows, reinterpret_cast<uint32_t*>(s));
-        tmem_wait_ld(reinterpret_cast<uint32_t*>(s));
+        float s[kMine];
+        tmem_ld16(tmem + lanes + b * kFewRows + from, reinterpret_cast<uint32_t*>(s));
+        tmem_wait_ld16(reinterpret_cast<uint32_t*>(s));
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&mi.s_free[b]);
-        if ((it.e.tile0 + j + 1) * kTile > least) {
+        uint32_t pk[kMine / 2];
+        if (mine) {
+          if ((it.e.tile0 + j + 1) * kTile > least) {
 #pragma unroll
-          for (int x = 0; x < kFewRows; ++x) s[x] = token < mi.limit[x] ? s[x] : -INFINITY;
-        }
-        float top = -INFINITY;
-#pragma unroll
-        for (int g = 0; g < kFewRows / 8; ++g) {
-          if (g >= groups) break;
-          const float4 o0 = *reinterpret_cast<const float4*>(&mi.off[g * 8]);
-          const float4 o1 = *reinterpret_cast<const float4*>(&mi.off[g * 8 + 4]);
-          const float o[8] = {o0.x, o0.y, o0.z, o0.w, o1.x, o1.y, o1.z, o1.w};
-#pragma unroll
-          for (int x = 0; x < 8; ++x) s[g * 8 + x] = fmaf(s[g * 8 + x], c, o[x]);
-#pragma unroll
-          for (int x = 0; x < 8; x += 2) top = max3(top, s[g * 8 + x], s[g * 8 + x + 1]);
-        }
-        if (any_of_128(j == 0 || top > kGrow)) {
-          // maxima of the tile's columns, relative to the references
-#pragma unroll
-          for (int x = 0; x < kFewRows; ++x) {
-            if (x >= rows) break;
-            float v;
-            asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(v) : "f"(s[x]));
-            if (lane == 0) mi.most[warp][x] = v;
+            for (int x = 0; x < kMine; ++x) s[x] = token < mi.limit[from + x] ? s[x] : -INFINITY;
           }
-          sync_128();
-          if (tid < kFewRows) {
-            float v = -INFINITY;
-            if (tid < rows) v = fmaxf(fmaxf(mi.most[0][tid], mi.most[1][tid]), fmaxf(mi.most[2][tid], mi.most[3][tid]));
-            const float by = j == 0 ? (v == -INFINITY ? 0.0f : v) : fmaxf(v, 0.0f);
-            mi.delta[tid] = by;
-            mi.factor[tid] = exp2f(-by);
-            mi.off[tid] -= by;
-          }
-          sync_128();
-          if (j > 0) {
-            wait(&mi.p_free, count - 1);  // the outputs so far are done
-            fence_after();
-#pragma unroll 1
-            for (int acc = kTmemO; acc <= kTmemL; acc += kFewRows) {
-#pragma unroll 1
-              for (int x0 = 0; x0 < kFewRows; x0 += 16) {
-                uint32_t o[16];
-                tmem_ld16(tmem + lanes + acc + x0, o);
-                tmem_wait_ld16(o);
+          float top = -INFINITY;
 #pragma unroll
-                for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * mi.factor[x0 + x]);
-                tmem_st16(tmem + lanes + acc + x0, o);
-              }
+          for (int g = 0; g < kMine / 8; ++g) {
+            if (g >= mine) break;
+            const float4 o0 = *reinterpret_cast<const float4*>(&mi.off[from + g * 8]);
+            const float4 o1 = *reinterpret_cast<const float4*>(&mi.off[from + g * 8 + 4]);
+            const float o[8] = {o0.x, o0.y, o0.z, o0.w, o1.x, o1.y, o1.z, o1.w};
+#pragma unroll
+            for (int x = 0; x < 8; ++x) s[g * 8 + x] = fmaf(s[g * 8 + x], c, o[x]);
+#pragma unroll
+            for (int x = 0; x < 8; x += 2) top = max3(top, s[g * 8 + x], s[g * 8 + x + 1]);
+          }
+          if (any_of_128(bar, j == 0 || top > kGrow)) {
+            // maxima of the tile's columns, relative to the references
+#pragma unroll
+            for (int x = 0; x < kMine; ++x) {
+              if (x >= held) break;
+              float v;
+              asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(v) : "f"(s[x]));
+              if (lane == 0) mi.most[warp & 3][from + x] = v;
             }
-            tmem_wait_st();
+            sync_128(bar);
+            if (tok128 < mine * 8) {
+              const int x = from + tok128;
+              float v = -INFINITY;
+              if (tok128 < held) v = fmaxf(fmaxf(mi.most[0][x], mi.most[1][x]), fmaxf(mi.most[2][x], mi.most[3][x]));
+              const float by = j == 0 ? (v == -INFINITY ? 0.0f : v) : fmaxf(v, 0.0f);
+              mi.delta[x] = by;
+              mi.factor[x] = exp2f(-by);
+              mi.off[x] -= by;
+            }
+            sync_128(bar);
+            if (j > 0) {
+              wait(&mi.p_free, count - 1);  // the outputs so far are done
+              fence_after();
+#pragma unroll 1
+              for (int x0 = 0; x0 < mine * 8; x0 += 4) {
+#pragma unroll 1
+                for (int acc = kTmemO; acc <= kTmemL; acc += kFewRows) {
+                  uint32_t o[4];
+                  tmem_ld4(tmem + lanes + acc + from + x0, o);
+                  tmem_wait_ld4(o);
+#pragma unroll
+                  for (int x = 0; x < 4; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * mi.factor[from + x0 + x]);
+                  tmem_st4(tmem + lanes + acc + from + x0, o);
+                }
+              }
+              tmem_wait_st();
+            }
+#pragma unroll
+            for (int x = 0; x < kMine; ++x)
+              if (x < mine * 8) s[x] -= mi.delta[from + x];
           }
 #pragma unroll
-          for (int x = 0; x < kFewRows; ++x) s[x] -= mi.delta[x];
-        }
-        uint32_t pk[kFewRows / 2];
+          for (int g = 0; g < kMine / 8; ++g) {
+            if (g >= mine) break;
 #pragma unroll
-        for (int g = 0; g < kFewRows / 8; ++g) {
-          if (g >= groups) break;
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            float p0, p1;
-            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p0) : "f"(s[g * 8 + 2 * x]));
-            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p1) : "f"(s[g * 8 + 2 * x + 1]));
-            pk[g * 4 + x] = as_u32(__floats2half2_rn(p0, p1));
+            for (int x = 0; x < 4; ++x) {
+              float p0, p1;
+              asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p0) : "f"(s[g * 8 + 2 * x]));
+              asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p1) : "f"(s[g * 8 + 2 * x + 1]));
+              pk[g * 4 + x] = as_u32(__floats2half2_rn(p0, p1));
+            }
           }
         }
         wait(&mi.p_free, count + 1);  // the product with the last tile's P is done
 #pragma unroll
-        for (int g = 0; g < kFewRows / 8; ++g) {
-          if (g >= groups) break;
-          *reinterpret_cast<uint4*>(sm + L::kP + tid * 64 + ((g ^ ((tid >> 1) & 3)) << 4)) =
+        for (int g = 0; g < kMine / 8; ++g) {
+          if (g >= mine) break;
+          *reinterpret_cast<uint4*>(sm + L::kP + tok128 * 64 + (((from / 8 + g) ^ ((tok128 >> 1) & 3)) << 4)) =
               make_uint4(pk[g * 4], pk[g * 4 + 1], pk[g * 4 + 2], pk[g * 4 + 3]);
         }
         fence_smem();
@@ -331,18 +343,18 @@ __global__ void __launch_bounds__(kFewThreads, 1) extend_few_kernel(const __grid
         if (lane == 0) mbar_arrive(&mi.p_full);
       }
 
-      // a thread per column of O as the accumulator has it, 4 rows at a time
+      // a thread per column of O as the accumulator has it, 4 rows at a time, dealt out to the warpgroups
       if (n) {
         wait(&mi.o_full, n_o);
         fence_after();
       }
       const BadList& bad = mi.bad[n_o % kBadLists];
       constexpr bool kPaired = VM == KNLP_KV_INT4_SYM || VM == KNLP_KV_INT4_ASYM;
-      const int d = kPaired ? (tid & ~7) + ((tid >> 1) & 3) + 4 * (tid & 1) : tid;
+      const int d = kPaired ? (tok128 & ~7) + ((tok128 >> 1) & 3) + 4 * (tok128 & 1) : tok128;
       const bool direct = it.e.part < 0;
       float* part = p.parts + (static_cast<int64_t>(it.e.part) + static_cast<int64_t>(it.head) * rows) * (D + 4);
 #pragma unroll 1
-      for (int x0 = 0; x0 < rows; x0 += 4) {
+      for (int x0 = wg * 4; x0 < rows; x0 += 8) {
         uint32_t ou[4], lu[4];
         if (n) {
           tmem_ld4(tmem + lanes + kTmemO + x0, ou);
@@ -355,34 +367,34 @@ __global__ void __launch_bounds__(kFewThreads, 1) extend_few_kernel(const __grid
         }
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const int r = x0 + x;
-          if (r >= rows) break;
+          const int row = x0 + x;
+          if (row >= rows) break;
           const float l = __uint_as_float(lu[x]);
           float v = __uint_as_float(ou[x]);
           if (direct) v *= l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
-          if (n && bad.count && bad.hits(mi.limit[r], d / 32)) v = NAN;  // never in a healthy cache
+          if (n && bad.count && bad.hits(mi.limit[row], d / 32)) v = NAN;  // never in a healthy cache
           if (direct) {
-            if (tid < D) store_elem_rt(a.out, mi.out_row[r] * a.out_row_stride + d, v, a.out_dtype);
-            if (tid == r && a.lse) a.lse[mi.out_row[r]] = l == 0.0f ? -INFINITY : kLn2 * (log2f(l) - mi.off[r]);
+            if (tok128 < D) store_elem_rt(a.out, mi.out_row[row] * a.out_row_stride + d, v, a.out_dtype);
+            if (tok128 == row && a.lse) a.lse[mi.out_row[row]] = l == 0.0f ? -INFINITY : kLn2 * (log2f(l) - mi.off[row]);
           } else {
-            if (tid < D) part[r * (D + 4) + d] = v;
+            if (tok128 < D) part[row * (D + 4) + d] = v;
             // a piece that holds nothing for the row does not weigh
-            if (tid == r) part[r * (D + 4) + D] = l == 0.0f ? -INFINITY : -mi.off[r], part[r * (D + 4) + D + 1] = l;
+            if (tok128 == row) part[row * (D + 4) + D] = l == 0.0f ? -INFINITY : -mi.off[row], part[row * (D + 4) + D + 1] = l;
           }
         }
       }
       fence_before();
       n_o += n > 0;
     }
-  } else if (warp < 20) {
-    const int wg = (warp - 4) >> 2;  // K, K, V, V
+  } else if (warp < 24) {
+    const int wg = (warp - 8) >> 2;  // K, K, V, V
     if constexpr (KM == VM && L::kStagesK == L::kStagesV) {
       few_produce<L, KM, D, L::kStagesK>(p, sm, mi, n_items, wg >> 1, wg & 1, warp & 3, lane);
     } else {
       if (wg < 2) few_produce<L, KM, D, L::kStagesK>(p, sm, mi, n_items, 0, wg, warp & 3, lane);
       else few_produce<L, VM, D, L::kStagesV>(p, sm, mi, n_items, 1, wg - 2, warp & 3, lane);
     }
-  } else if (warp < 22) {
+  } else if (warp < 26) {
     // ---------------------------------------------------------------- matrix products
     auto wait_warp = [&](uint64_t* x, uint32_t phase) { mbar_wait_warp(x, phase & 1, &mi.abort, p.status); };
     const uint32_t tm = uniform(tmem);
@@ -392,7 +404,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) extend_few_kernel(const __grid
       const Item it(p, k);
       const int n = uniform(it.tiles());
       if (n == 0) continue;
-      if (warp == 20) {
+      if (warp == 24) {
         const uint32_t idesc = product(kTile, kFewRows, KM == kRaw && a.k.mode == KNLP_KV_BF16, false);
         const uint32_t q = operand(smem_addr(sm + L::kQ), 16);
         wait_warp(&mi.q_full, n_q++);
@@ -448,7 +460,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) extend_few_kernel(const __grid
   fence_before();
   __syncthreads();
   fence_after();
-  if (warp == 20)
+  if (warp == 24)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmemColumns) : "memory");
 }
 
