@@ -21,6 +21,7 @@
 
 #include <cooperative_groups.h>
 
+#include "pair_math.cuh"
 #include "serve.cuh"
 
 namespace cg = cooperative_groups;
@@ -28,16 +29,16 @@ namespace cg = cooperative_groups;
 namespace knlp {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kGroups = kThreads / 4;  // shares of four neighbouring threads
+constexpr int kGroups = kThreads / 2;  // shares of two neighbouring threads
 constexpr int kCap = 1024;             // collected candidates of one slice
 constexpr int kMaxTop = KNLP_MAX_TOP;
 constexpr int kMaxParts = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-static_assert(kMaxParts * kMaxTop <= kThreads && kThreads <= kCap, "one candidate per thread");
+static_assert(kMaxParts * kMaxTop <= kCap, "");
 
 struct ScoreArgs {
   const void* logits;
@@ -61,7 +62,8 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // Exponent of 2^.. for a difference of logits that is <= 0.  Differences are formed before they
 // are scaled (masks may be the type's lowest value, whose product with log2 e overflows); -1e4
 // stands for every exponent that gives 0, so that a masked logit adds 0 and not 0 * inf.
-__device__ __forceinline__ float exponent(float diff) { return max_nan(diff * kLog2e, -1e4f); }
+constexpr float kNothing = -1e4f;
+__device__ __forceinline__ float exponent(float diff) { return max_nan(diff * kLog2e, kNothing); }
 
 // Order of the values: NaN above +inf, -0 equal to +0.
 __device__ __forceinline__ uint32_t order(float x) {
@@ -139,27 +141,44 @@ struct Vec<KNLP_BF16> {
   }
 };
 
+// A thread's running statistics: its sums in two halves, for paired arithmetic.
+struct Running {
+  float m = -INFINITY;
+  uint64_t l = 0, w = 0;
+  int above = 0;
+  __device__ __forceinline__ Stats total() const {
+    float l0, l1, w0, w1;
+    unpack2(l, l0, l1);
+    unpack2(w, w0, w1);
+    return {m, l0 + l1, w0 + w1, above};
+  }
+};
+
+// N (even) values, or one (the other half of its pair a masked logit).
 template <int N>
-__device__ __forceinline__ void take(Stats& s, const float* f, float given) {
+__device__ __forceinline__ void take(Running& s, const float* f, float given) {
   float c = f[0];
 #pragma unroll
   for (int i = 1; i < N; ++i) c = max_nan(c, f[i]);
   if (!(c <= s.m)) {  // also for a NaN, which then stays
-    if (s.l != 0.0f) {
+    if (s.m != -INFINITY) {
       const float d = exponent(s.m - c), e = exp2f(d);
-      s.w = (s.w + d * s.l) * e;
-      s.l *= e;
+      s.w = mul2(fma2(pack2(d, d), s.l, s.w), pack2(e, e));
+      s.l = mul2(s.l, pack2(e, e));
     }
     s.m = max_nan(s.m, c);
   }
   if (s.m == -INFINITY) return;
+  const uint64_t off = pack2(-s.m, -s.m), scale = pack2(kLog2e, kLog2e);
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float t = exponent(f[i] - s.m);
-    float e;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-    s.l += e;
-    s.w = fmaf(e, t, s.w);
+  for (int i = 0; i < N; i += 2) {
+    float t0, t1, e0, e1;
+    unpack2(mul2(add2(pack2(f[i], i + 1 < N ? f[i + 1] : -INFINITY), off), scale), t0, t1);
+    t0 = max_nan(t0, kNothing), t1 = max_nan(t1, kNothing);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(t0));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(t1));
+    s.l = add2(s.l, pack2(e0, e1));
+    s.w = fma2(pack2(e0, e1), pack2(t0, t1), s.w);
   }
   if (!(c <= given)) {
 #pragma unroll
@@ -241,8 +260,7 @@ __device__ void top_of_slice(Shared& sh, const Slice<DT>& s, int k, float share_
   if (tid == 0) sh.n_cand = sh.n_strict = sh.n_hot = sh.ties = 0;
   float g = share_max;
   g = max_nan(g, __shfl_xor_sync(~0u, g, 1));
-  g = max_nan(g, __shfl_xor_sync(~0u, g, 2));
-  if ((tid & 3) == 0) sh.group[tid >> 2] = order(g);
+  if ((tid & 1) == 0) sh.group[tid >> 1] = order(g);
   __syncthreads();
   // the k-th largest group maximum (k <= kMaxTop < kGroups)
   if (tid < kGroups) {
@@ -344,13 +362,13 @@ __global__ void __launch_bounds__(kThreads) token_score_kernel(ScoreArgs a) {
   const bool known = id >= 0 && id < a.vocab;
   const float given = known ? load_elem<DT>(x, id) : INFINITY;
 
-  Stats st{-INFINITY, 0.0f, 0.0f, 0};
+  Running run;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     const int i = s.single(tid, which);
     if (i >= 0) {
       const float f = s.at(i);
-      take<1>(st, &f, given);
+      take<1>(run, &f, given);
     }
   }
   int v = tid;
@@ -362,16 +380,17 @@ __global__ void __launch_bounds__(kThreads) token_score_kernel(ScoreArgs a) {
     for (int j = 0; j < 4; ++j) {
       float f[N];
       Vec<DT>::unpack(u[j], f);
-      take<N>(st, f, given);
+      take<N>(run, f, given);
     }
   }
   for (; v < s.vecs; v += kThreads) {
     float f[N];
     Vec<DT>::unpack(s.vec(v), f);
-    take<N>(st, f, given);
+    take<N>(run, f, given);
   }
 
-  const float share_max = st.m;
+  const float share_max = run.m;
+  Stats st = run.total();
   merge_lanes(st, 32);
   if (lane == 0) sh.warp[warp] = st;
   if (a.top_k) top_of_slice<DT>(sh, s, a.top_k, share_max);
@@ -388,8 +407,8 @@ __global__ void __launch_bounds__(kThreads) token_score_kernel(ScoreArgs a) {
       merge_lanes(all, parts);
       if (lane == 0) sh.warp[0] = all;
     }
-    const int n = parts * a.top_k;  // <= kThreads
-    if (tid < n) sh.cand[tid] = cluster.map_shared_rank(&sh, tid / a.top_k)->top[tid % a.top_k];
+    const int n = parts * a.top_k;  // <= kCap
+    for (int i = tid; i < n; i += kThreads) sh.cand[i] = cluster.map_shared_rank(&sh, i / a.top_k)->top[i % a.top_k];
     __syncthreads();
     const Stats t = sh.warp[0];
     const bool empty = t.m == -INFINITY;  // no logit above -inf: no token has a probability
@@ -400,8 +419,8 @@ __global__ void __launch_bounds__(kThreads) token_score_kernel(ScoreArgs a) {
       a.entropy[row] = empty ? 0.0f : log_sum - kLn2 * (t.w / t.l);
       a.rank[row] = known ? t.above + 1 : 0;
     }
-    if (tid < n) {
-      const uint64_t mine = sh.cand[tid];
+    for (int i = tid; i < n; i += kThreads) {
+      const uint64_t mine = sh.cand[i];
       int before = 0;
       for (int j = 0; j < n; ++j) before += sh.cand[j] > mine;
       if (before < a.top_k && mine) sh.merged[before] = mine;
