@@ -11,6 +11,7 @@ bit-identical codes and scales.  CUDA tensors only: there is no CPU path.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import time
 from abc import ABC, abstractmethod
@@ -146,6 +147,16 @@ class CompressionBackend(ABC):
                    device_str: str, max_ctx: int) -> Tuple[torch.Tensor, List[V14StepStats]]:
         """Prefill on ``prefix_ids`` then feed ``continuation_ids`` one token at a time.
         Returns (logits [B, decode_steps + 1, V], one V14StepStats per decode step)."""
+
+    def run_score(self, model, prefix_ids: torch.Tensor, continuation_ids: torch.Tensor,
+                  device_str: str, max_ctx: int, top_k: int = 0):
+        """How likely the continuation is after the prefix, under this backend's cache: what the
+        harness computes from ``run_decode``'s logits (its compute_ppl).  Returns
+        (``scoring.TokenScores`` of the continuation's tokens [B, n], the step statistics); the
+        perplexity is ``(-scores.logprob.mean()).exp()``."""
+        from . import scoring
+        logits, stats = self.run_decode(model, prefix_ids, continuation_ids, device_str, max_ctx)
+        return scoring.token_logprobs(logits[:, :-1], continuation_ids, top_k), stats
 
     def compression_ratio(self) -> float:
         return 1.0
@@ -369,39 +380,56 @@ _ATTN_NAME = "knlp_b200_packed"
 
 def _packed_attention(module, query, key, value, attention_mask=None, dropout=0.0, scaling=None,
                       **kwargs):
-    """Attention function installed into the model while ``PackedQuantBackend.run_decode``
-    steps: ``key`` / ``value`` hold only the tokens kept in full (sink + near + new), the
-    far tokens of this layer live in a packed cache and are attended to by the decode
-    kernel; the two softmax partials are merged by the combine kernel."""
+    """Attention function installed into the model while ``PackedQuantBackend`` steps through a
+    continuation, one token or a chunk at a time: ``key`` / ``value`` hold only the tokens kept in
+    full (sink + near + new), the far tokens of this layer live in a packed cache and are attended
+    to by the decode kernel (several new tokens: the extend kernel); the two softmax partials are
+    merged by the combine kernel."""
     from . import ops
     st = _ACTIVE_PACKED
-    if st is None or query.shape[2] != 1:
-        raise RuntimeError("the packed attention function only serves single-token decode steps "
-                           "of PackedQuantBackend.run_decode")
-    B, H, _, D = query.shape
+    if st is None:
+        raise RuntimeError("the packed attention function only serves the steps of "
+                           "PackedQuantBackend.run_decode / run_score")
+    B, H, T, D = query.shape
     if scaling is not None and abs(scaling - D ** -0.5) > 1e-6 * D ** -0.5:
         raise NotImplementedError("only the standard head_dim^-1/2 softmax scale is supported")
     far = st._far[module.layer_idx]
-    q3 = query.reshape(B, H, D).contiguous()
-    # dense part (sink + near + the new token): one partial (o un-normalised, m, l) per row
+    q = query.transpose(1, 2).reshape(B * T, H, D).contiguous()  # rows (sequence, token)
+    # dense part (sink + near + the new tokens up to the row's own): one partial
+    # (o un-normalised, m, l) per row
     n_rep = H // key.shape[1]
     k = key if n_rep == 1 else key.repeat_interleave(n_rep, dim=1)
     v = value if n_rep == 1 else value.repeat_interleave(n_rep, dim=1)
-    s = torch.einsum("bhd,bhtd->bht", q3.float(), k.float()) * (D ** -0.5)
+    s = torch.einsum("bthd,bhkd->bthk", q.view(B, T, H, D).float(), k.float()) * (D ** -0.5)
+    if T > 1:
+        n = k.shape[2]
+        later = torch.arange(n, device=s.device)[None] > torch.arange(n - T, n, device=s.device)[:, None]
+        s.masked_fill_(later[None, :, None], float("-inf"))
     m = s.max(dim=-1, keepdim=True).values
     pr = torch.exp(s - m)
-    dense = torch.cat([torch.einsum("bht,bhtd->bhd", pr, v.float()), m,
-                       pr.sum(dim=-1, keepdim=True)], dim=-1)
+    dense = torch.cat([torch.einsum("bthk,bhkd->bthd", pr, v.float()), m,
+                       pr.sum(dim=-1, keepdim=True)], dim=-1).view(B * T, H, D + 2)
     if far is None:
         packed = dense.unsqueeze(0)
     else:
         cache, table, lens = far
-        far_part = ops.decode_attention(q3, cache._k_plane(), cache._v_plane(), cache.num_blocks,
-                                        table, lens, cache.num_kv_heads, D, cache.block_size,
-                                        max_seq_len=st._n_far, emit_partial=True)
-        packed = torch.stack([far_part, dense.contiguous()])
+        if T == 1 or q.dtype == torch.float32:
+            # one row per token; fp32 queries keep their precision in the decode kernel only
+            far_part = ops.decode_attention(q, cache._k_plane(), cache._v_plane(), cache.num_blocks,
+                                            table if T == 1 else table.repeat_interleave(T, 0),
+                                            lens if T == 1 else lens.repeat_interleave(T),
+                                            cache.num_kv_heads, D, cache.block_size,
+                                            max_seq_len=st._n_far, emit_partial=True)
+        else:
+            starts = torch.arange(0, B * T + 1, T, dtype=torch.int32, device=q.device)
+            o, lse = ops.extend_attention(
+                q, cache._k_plane(), cache._v_plane(), cache.num_blocks, table, lens, starts,
+                cache.num_kv_heads, D, cache.block_size, causal=False, max_query_len=T,
+                max_seq_len=st._n_far, out_dtype=torch.float32, return_lse=True)
+            far_part = torch.cat([o, lse[..., None], torch.ones_like(lse)[..., None]], dim=-1)
+        packed = torch.stack([far_part, dense])
     out = ops.combine_packed(packed.contiguous(), out_dtype=query.dtype)
-    return out.view(B, 1, H, D), None
+    return out.view(B, T, H, D), None
 
 
 class PackedQuantBackend(QuantBackend):
@@ -464,45 +492,83 @@ class PackedQuantBackend(QuantBackend):
                 total += n_compressed * c.expected_bytes_per_block() // c.block_size
         return int(total)
 
-    @torch.no_grad()
-    def run_decode(self, model, prefix_ids, continuation_ids, device_str, max_ctx):
+    @contextlib.contextmanager
+    def _installed(self, model):
+        """The packed attention in the model's layers."""
         global _ACTIVE_PACKED
         from transformers import AttentionInterface
 
-        n_layers = self.mc["n_layers"]
-        bpt = _kv_bytes_per_token(self.mc)
-        out = model(prefix_ids, use_cache=True)
-        past = out.past_key_values
-        dtype = _layer_kv(past, 0)[0].dtype
-        logits = [out.logits[:, -1:, :]]
-        stats = []
-        pos = prefix_ids.shape[1]
-        t0 = time.perf_counter()
-        past, n_full, n_compressed = self._pack_far(past, dtype)
-        compress_ms = (time.perf_counter() - t0) * 1000
         AttentionInterface.register(_ATTN_NAME, _packed_attention)
         old_impl = model.config._attn_implementation
         _ACTIVE_PACKED = self
         try:
             model.config._attn_implementation = _ATTN_NAME
-            for step in range(continuation_ids.shape[1]):
-                pos_ids = torch.tensor([[pos]], device=device_str, dtype=torch.long)
-                out = model(continuation_ids[:, step:step + 1], past_key_values=past,
-                            use_cache=True, position_ids=pos_ids)
-                past = out.past_key_values
-                logits.append(out.logits)
-                pos += 1
-                bytes_full = (n_full + step + 1) * bpt * n_layers
-                bytes_comp = self._compressed_bytes(n_compressed)
-                stats.append(V14StepStats(
-                    kv_kept=n_full + step + 1 + n_compressed, kv_bytes_full=bytes_full,
-                    kv_bytes_compressed=bytes_comp, kv_bytes_total=bytes_full + bytes_comp,
-                    compress_ms=compress_ms if step == 0 else 0,
-                    n_full=n_full + step + 1, n_compressed=n_compressed))
+            yield
         finally:
             model.config._attn_implementation = old_impl
             _ACTIVE_PACKED = None
-        return torch.cat(logits, dim=1), stats
+
+    @torch.no_grad()
+    def _steps(self, model, prefix_ids, continuation_ids, device_str, chunk):
+        """Prefill on the prefix, pack the far tokens, then the continuation, ``chunk`` tokens a
+        step.  Yields (logits of the step, statistics or None for the prefill)."""
+        n_layers = self.mc["n_layers"]
+        bpt = _kv_bytes_per_token(self.mc)
+        out = model(prefix_ids, use_cache=True)
+        past = out.past_key_values
+        dtype = _layer_kv(past, 0)[0].dtype
+        pos = prefix_ids.shape[1]
+        t0 = time.perf_counter()
+        past, n_full, n_compressed = self._pack_far(past, dtype)
+        compress_ms = (time.perf_counter() - t0) * 1000
+        yield out.logits[:, -1:, :], None
+        with self._installed(model):
+            for at in range(0, continuation_ids.shape[1], chunk):
+                ids = continuation_ids[:, at:at + chunk]
+                pos_ids = torch.arange(pos, pos + ids.shape[1], device=device_str)[None]
+                out = model(ids, past_key_values=past, use_cache=True, position_ids=pos_ids)
+                past = out.past_key_values
+                pos += ids.shape[1]
+                done = at + ids.shape[1]
+                bytes_full = (n_full + done) * bpt * n_layers
+                bytes_comp = self._compressed_bytes(n_compressed)
+                yield out.logits, V14StepStats(
+                    kv_kept=n_full + done + n_compressed, kv_bytes_full=bytes_full,
+                    kv_bytes_compressed=bytes_comp, kv_bytes_total=bytes_full + bytes_comp,
+                    compress_ms=compress_ms if at == 0 else 0,
+                    n_full=n_full + done, n_compressed=n_compressed)
+
+    def run_decode(self, model, prefix_ids, continuation_ids, device_str, max_ctx):
+        with contextlib.closing(
+                self._steps(model, prefix_ids, continuation_ids, device_str, 1)) as steps:
+            logits, stats = zip(*steps)
+        return torch.cat(logits, dim=1), list(stats[1:])
+
+    def run_score(self, model, prefix_ids, continuation_ids, device_str, max_ctx, top_k=0,
+                  chunk: int = 256):
+        """As the base class, with ``chunk`` tokens of the continuation a step instead of one (the
+        new tokens attend to the packed far segment through the extend kernel) and one step's
+        logits at a time.  One ``V14StepStats`` per chunk."""
+        from . import scoring
+        if chunk < 1:
+            raise ValueError("chunk must be at least 1")
+        parts, stats, at = [], [], 0
+        n = continuation_ids.shape[1]
+        steps = self._steps(model, prefix_ids, continuation_ids, device_str, chunk)
+        with contextlib.closing(steps):  # the model gets its attention back, whatever happens
+            for logits, st in steps:
+                if st is not None:
+                    stats.append(st)
+                # what predicts token `at`: the prefill's last row, then all but the very last
+                rows = logits[:, :min(logits.shape[1], n - at)]
+                if rows.shape[1]:
+                    ids = continuation_ids[:, at:at + rows.shape[1]]
+                    parts.append(scoring.token_logprobs(rows, ids, top_k))
+                    at += rows.shape[1]
+        if not parts:
+            return scoring.token_logprobs(logits[:, :0], continuation_ids, top_k), stats
+        cat = [None if f[0] is None else torch.cat(f, dim=1) for f in zip(*parts)]
+        return scoring.TokenScores(*cat), stats
 
     def description(self):
         return "packed far cache: " + super().description()

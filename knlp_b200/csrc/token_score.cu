@@ -441,6 +441,8 @@ int launch_token_score(const void* logits, int dtype, int64_t row_stride, const 
                        int n_rows, int vocab, int top_k, float* logprob, float* entropy,
                        int32_t* rank, int64_t* top_ids, float* top_logprobs, int n_sms,
                        cudaStream_t st) {
+  // Slices while they find idle SMs: with two blocks per SM 128 rows of 128256 bf16 logits take 20.5
+  // us (2 slices each), with eight 29.6 us (8 slices): a block's own ranking does not get shorter.
   int parts = 1;
   while (parts < kMaxParts && n_rows * parts * 2 <= n_sms * 2 && vocab / (parts * 2) >= 4096)
     parts *= 2;
