@@ -170,13 +170,16 @@ class AttentionMetadataBuilder:
     def build_from_lengths(self, context_lens: torch.Tensor, query_lens: torch.Tensor,
                            block_table: torch.Tensor, free_blocks: torch.Tensor, *,
                            num_tokens: int, max_query_len: int, max_seq_len: int,
+                           padded_tokens: Optional[int] = None,
                            free_head: Optional[torch.Tensor] = None
                            ) -> Tuple[AttentionMetadata, StepTables]:
         """Metadata of a step whose tables are built here (``build_step``) instead of taken
         ready-made: the block table is updated in place.  ``num_tokens``, ``max_query_len``,
-        ``max_seq_len``: the host's counts of the step."""
+        ``max_seq_len``: the host's counts of the step; ``padded_tokens``: rows of the slot
+        mapping where a step is padded to a fixed size."""
         t = build_step(context_lens, query_lens, block_table, free_blocks, self.block_size,
-                       num_tokens, free_head=free_head)
+                       num_tokens if padded_tokens is None else padded_tokens,
+                       free_head=free_head)
         return AttentionMetadata(
             num_actual_tokens=num_tokens, max_query_len=max_query_len,
             query_start_loc=t.query_start_loc, max_seq_len=max_seq_len, seq_lens=t.seq_lens,

@@ -9,7 +9,7 @@ namespace extend {
 // One pair of plane modes, both head dimensions: the kernel for many rows on `many`, then the one
 // for few rows on `few`, each a programmatic dependent of the launch before it.
 template <int KM, int VM>
-int launch_extend_pair(const Params& many, const Params& few, int grid, cudaStream_t st);
+int launch_extend_pair(const Params& many, const Params& few, bool only_few, int grid, cudaStream_t st);
 
 inline int launch_dependent(void (*fn)(Params), const Params& p, int grid, int threads, int smem, cudaStream_t st) {
   if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
@@ -34,21 +34,22 @@ inline int launch_dependent(void (*fn)(Params), const Params& p, int grid, int t
 }
 
 template <int KM, int VM, int D>
-int launch_extend_one(const Params& many, const Params& few, int grid, cudaStream_t st) {
-  const int rc = launch_dependent(extend_mma_kernel<KM, VM, D>, many, grid, kThreads, Layout<KM, VM, D>::kBytes, st);
+int launch_extend_one(const Params& many, const Params& few, bool only_few, int grid, cudaStream_t st) {
+  const int rc = only_few ? KNLP_OK : launch_dependent(extend_mma_kernel<KM, VM, D>, many, grid, kThreads, Layout<KM, VM, D>::kBytes, st);
   if (rc) return rc;
   return launch_dependent(few::extend_few_kernel<KM, VM, D>, few, grid, few::kFewThreads, few::FewLayout<KM, VM, D>::kBytes, st);
 }
 
-#define KNLP_EXTEND_PAIR(KM, VM)                                                                       \
-  namespace knlp {                                                                                     \
-  namespace extend {                                                                                   \
-  template <>                                                                                          \
-  int launch_extend_pair<KM, VM>(const Params& many, const Params& few, int grid, cudaStream_t st) {   \
-    return many.a.head_dim == 64 ? launch_extend_one<KM, VM, 64>(many, few, grid, st)                  \
-                                 : launch_extend_one<KM, VM, 128>(many, few, grid, st);                \
-  }                                                                                                    \
-  }                                                                                                    \
+#define KNLP_EXTEND_PAIR(KM, VM)                                                              \
+  namespace knlp {                                                                            \
+  namespace extend {                                                                          \
+  template <>                                                                                 \
+  int launch_extend_pair<KM, VM>(const Params& many, const Params& few, bool only_few,        \
+                                 int grid, cudaStream_t st) {                                 \
+    return many.a.head_dim == 64 ? launch_extend_one<KM, VM, 64>(many, few, only_few, grid, st)   \
+                                 : launch_extend_one<KM, VM, 128>(many, few, only_few, grid, st); \
+  }                                                                                           \
+  }                                                                                           \
   }
 
 }  // namespace extend

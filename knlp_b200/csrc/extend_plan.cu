@@ -19,6 +19,7 @@ namespace {
 constexpr int kPlanThreads = 512;
 constexpr int kCandidates = kPlanThreads / 32;
 constexpr int kMaxRows = 2 * kRows;
+constexpr int kSharedSeqs = 1024, kSharedTiles = 2048;
 // Time of an item in units of one 128 x 128 tile of one stream: what it costs besides its tiles
 // (query in, result out, an empty pipeline at both ends), and of the merging launch.
 constexpr float kItemCost = 4.0f, kMergeCost = 5.0f;
@@ -116,7 +117,10 @@ extend_plan_kernel(const __grid_constant__ ExtendArgs a, int rep, int n_ctas, co
                    const __grid_constant__ Lists few) {
   const bool few_rows = blockIdx.x;  // a block per kernel
   const Lists& to = few_rows ? few : many;
-  int* const base = to.base;
+  // small batches are planned out of shared memory: every step of it is a latency
+  __shared__ int sh_base[kSharedSeqs + 1];
+  __shared__ int2 sh_tiles[kSharedTiles];  // (kv, rows)
+  int* const base = a.n_seqs <= kSharedSeqs ? sh_base : to.base;
   __shared__ int sh[4][kPlanThreads / 32];
   __shared__ float sh_cost[kCandidates], sh_piece[kCandidates], sh_worst[kCandidates];
   __shared__ int sh_at[kPlanThreads];
@@ -139,7 +143,18 @@ extend_plan_kernel(const __grid_constant__ ExtendArgs a, int rep, int n_ctas, co
   n_tiles = min(n_tiles, to.max_tiles);  // more only for offsets that are not ascending
 
   float cost = 0.0f;
-  for (int t = tid; t < n_tiles; t += kPlanThreads) cost += tile_at(a, few_rows, rep, base, t).cost();
+  for (int t = tid; t < n_tiles; t += kPlanThreads) {
+    const Tile x = tile_at(a, few_rows, rep, base, t);
+    cost += x.cost();
+    if (t < kSharedTiles) sh_tiles[t] = make_int2(x.kv, x.rows);
+  }
+  // a tile as far as its cost goes
+  auto size_of = [&](int t) {
+    if (t >= kSharedTiles) return tile_at(a, few_rows, rep, base, t);
+    Tile x{};
+    x.kv = sh_tiles[t].x, x.rows = sh_tiles[t].y;
+    return x;
+  };
 #pragma unroll
   for (int d = 16; d; d >>= 1) cost += __shfl_xor_sync(~0u, cost, d);
   if (lane == 0) sh_cost[warp] = cost;
@@ -155,7 +170,7 @@ extend_plan_kernel(const __grid_constant__ ExtendArgs a, int rep, int n_ctas, co
   int items = 0;
   int64_t parts = 0;
   for (int t = lane; t < n_tiles; t += 32) {
-    const Tile x = tile_at(a, few_rows, rep, base, t);
+    const Tile x = size_of(t);
     const int n = x.pieces(piece);
     items += n;
     worst = fmaxf(worst, x.cost() / n);
@@ -194,7 +209,7 @@ extend_plan_kernel(const __grid_constant__ ExtendArgs a, int rep, int n_ctas, co
   sh_at[tid] = 0;
   __syncthreads();
   for (int t = tid; t < n_tiles; t += kPlanThreads) {
-    const Tile x = tile_at(a, few_rows, rep, base, t);
+    const Tile x = size_of(t);
     const int n = x.pieces(c);
     atomicAdd(&sh_at[class_of(x, n)], n);
   }
@@ -307,16 +322,16 @@ bool plane_aligned(const Plane& p, int head_dim) {
   return rows(p.scales, p.ss) && (p.mode != KNLP_KV_INT4_ASYM || rows(p.zeros, p.zs));
 }
 
-int launch_modes(const Params& p, const Params& few, int grid, cudaStream_t st) {
+int launch_modes(const Params& p, const Params& few, bool only_few, int grid, cudaStream_t st) {
   const int k = p.a.k.mode == KNLP_KV_BF16 ? kRaw : p.a.k.mode, v = p.a.v.mode;
-  if (k == KNLP_KV_INT4_ASYM && v == KNLP_KV_INT4_ASYM) return launch_extend_pair<KNLP_KV_INT4_ASYM, KNLP_KV_INT4_ASYM>(p, few, grid, st);
-  if (k == KNLP_KV_INT4_SYM && v == KNLP_KV_INT4_SYM) return launch_extend_pair<KNLP_KV_INT4_SYM, KNLP_KV_INT4_SYM>(p, few, grid, st);
-  if (k == KNLP_KV_INT8_G32 && v == KNLP_KV_INT4_ASYM) return launch_extend_pair<KNLP_KV_INT8_G32, KNLP_KV_INT4_ASYM>(p, few, grid, st);
-  if (k == KNLP_KV_INT8_G32 && v == KNLP_KV_INT4_SYM) return launch_extend_pair<KNLP_KV_INT8_G32, KNLP_KV_INT4_SYM>(p, few, grid, st);
-  if (k == KNLP_KV_INT8_G32 && v == KNLP_KV_INT8_G32) return launch_extend_pair<KNLP_KV_INT8_G32, KNLP_KV_INT8_G32>(p, few, grid, st);
-  if (k == kRaw && v == KNLP_KV_INT4_ASYM) return launch_extend_pair<kRaw, KNLP_KV_INT4_ASYM>(p, few, grid, st);
-  if (k == kRaw && v == KNLP_KV_INT4_SYM) return launch_extend_pair<kRaw, KNLP_KV_INT4_SYM>(p, few, grid, st);
-  if (k == kRaw && v == KNLP_KV_INT8_G32) return launch_extend_pair<kRaw, KNLP_KV_INT8_G32>(p, few, grid, st);
+  if (k == KNLP_KV_INT4_ASYM && v == KNLP_KV_INT4_ASYM) return launch_extend_pair<KNLP_KV_INT4_ASYM, KNLP_KV_INT4_ASYM>(p, few, only_few, grid, st);
+  if (k == KNLP_KV_INT4_SYM && v == KNLP_KV_INT4_SYM) return launch_extend_pair<KNLP_KV_INT4_SYM, KNLP_KV_INT4_SYM>(p, few, only_few, grid, st);
+  if (k == KNLP_KV_INT8_G32 && v == KNLP_KV_INT4_ASYM) return launch_extend_pair<KNLP_KV_INT8_G32, KNLP_KV_INT4_ASYM>(p, few, only_few, grid, st);
+  if (k == KNLP_KV_INT8_G32 && v == KNLP_KV_INT4_SYM) return launch_extend_pair<KNLP_KV_INT8_G32, KNLP_KV_INT4_SYM>(p, few, only_few, grid, st);
+  if (k == KNLP_KV_INT8_G32 && v == KNLP_KV_INT8_G32) return launch_extend_pair<KNLP_KV_INT8_G32, KNLP_KV_INT8_G32>(p, few, only_few, grid, st);
+  if (k == kRaw && v == KNLP_KV_INT4_ASYM) return launch_extend_pair<kRaw, KNLP_KV_INT4_ASYM>(p, few, only_few, grid, st);
+  if (k == kRaw && v == KNLP_KV_INT4_SYM) return launch_extend_pair<kRaw, KNLP_KV_INT4_SYM>(p, few, only_few, grid, st);
+  if (k == kRaw && v == KNLP_KV_INT8_G32) return launch_extend_pair<kRaw, KNLP_KV_INT8_G32>(p, few, only_few, grid, st);
   return 1;
 }
 
@@ -391,7 +406,9 @@ int launch_extend_mma(const ExtendArgs& a, float* ws, int64_t ws_floats, int n_s
   }
   extend_plan_kernel<<<2, kPlanThreads, 0, st>>>(a, p[0].rep, n_sms, lists[0], lists[1]);
   if (cudaGetLastError() != cudaSuccess) return KNLP_ERR_LAUNCH;
-  const int rc = launch_modes(p[0], p[1], n_sms, st);
+  // with at most 32 rows in all no sequence has more
+  const bool only_few = static_cast<int64_t>(a.n_tokens) * p[0].rep <= few::kFewRows;
+  const int rc = launch_modes(p[0], p[1], only_few, n_sms, st);
   if (rc != KNLP_OK) return rc > 0 ? KNLP_ERR_MODE : rc;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(2 * n_sms);

@@ -707,7 +707,9 @@ def _extend_workspace(dev: torch.device, S: int, T: int, Hq: int, Hkv: int, d: i
         if len(_extend_sizes) >= 4096:
             _extend_sizes.clear()
         need = _extend_sizes[shape] = nf.value
-    if torch.cuda.is_current_stream_capturing():
+    with _on(dev):
+        capturing = torch.cuda.is_current_stream_capturing()
+    if capturing:
         return torch.empty(need, dtype=torch.float32, device=dev)
     key = (dev.index, _stream(dev))
     cur = _extend_ws.get(key)

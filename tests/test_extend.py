@@ -226,6 +226,29 @@ def test_ragged_batches(cuda_device):
 
 
 @pytest.mark.gpu
+def test_many_sequences_and_many_tiles(cuda_device):
+    """More sequences and more row tiles than the planning keeps in shared memory."""
+    rng = random.Random(5)
+    S = 1300
+    Batch(cuda_device, [rng.randint(0, 60) for _ in range(S)], [rng.choice((0, 1, 1, 1, 9)) for _ in range(S)],
+          8, 2, 64, "int4_asym", seed=31).check()
+    Batch(cuda_device, [rng.randint(0, 90) for _ in range(30)], [150] * 30, 128, 1, 64, "k8v8", seed=32).check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv", [(8, 1), (4, 4), (32, 2)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_row_counts_around_the_kernels_border(d, hq, hkv, cuda_device):
+    """Rows per kv head (new tokens x q heads of a group) around 8, 16, 24, 32, 128 and 256, where the
+    groups of the few-row kernel, the kernels and the tiles change."""
+    rep = hq // hkv
+    new = sorted({max(1, n // rep + k) for n in (8, 16, 24, 32, 128, 256, 288) for k in (-1, 0, 1)})
+    rng = random.Random(d)
+    Batch(cuda_device, [rng.choice((0, 5, 127, 300, 900)) for _ in new], new, hq, hkv, d, "int4_asym",
+          seed=33).check(out_dtype=torch.float32)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("generic", GENERIC)
 def test_full_and_scale(generic, cuda_device):
     """Every query token over all cached tokens; other scales than head_dim^-1/2."""
