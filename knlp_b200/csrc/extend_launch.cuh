@@ -1,6 +1,8 @@
 // Launches of the two tensor-core extend kernels for a pair of plane modes.
 #pragma once
 
+#include <atomic>
+
 #include "extend_few.cuh"
 
 namespace knlp {
@@ -11,10 +13,22 @@ namespace extend {
 template <int KM, int VM>
 int launch_extend_pair(const Params& many, const Params& few, bool only_few, int grid, cudaStream_t st);
 
-inline int launch_dependent(void (*fn)(Params), const Params& p, int grid, int threads, int smem, cudaStream_t st) {
-  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+template <auto FN>
+int launch_dependent(const Params& p, int grid, int threads, int smem, cudaStream_t st) {
+  // the attribute is set once per device (a bit each)
+  static std::atomic<uint64_t> ready{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
     cudaGetLastError();
     return KNLP_ERR_NO_DEVICE;
+  }
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (!(ready.load(std::memory_order_acquire) & bit)) {
+    if (cudaFuncSetAttribute(FN, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+      cudaGetLastError();
+      return KNLP_ERR_NO_DEVICE;
+    }
+    ready.fetch_or(bit, std::memory_order_release);
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
@@ -26,7 +40,7 @@ inline int launch_dependent(void (*fn)(Params), const Params& p, int grid, int t
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, fn, p) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, FN, p) != cudaSuccess) {
     cudaGetLastError();
     return KNLP_ERR_LAUNCH;
   }
@@ -35,9 +49,9 @@ inline int launch_dependent(void (*fn)(Params), const Params& p, int grid, int t
 
 template <int KM, int VM, int D>
 int launch_extend_one(const Params& many, const Params& few, bool only_few, int grid, cudaStream_t st) {
-  const int rc = only_few ? KNLP_OK : launch_dependent(extend_mma_kernel<KM, VM, D>, many, grid, kThreads, Layout<KM, VM, D>::kBytes, st);
+  const int rc = only_few ? KNLP_OK : launch_dependent<extend_mma_kernel<KM, VM, D>>(many, grid, kThreads, Layout<KM, VM, D>::kBytes, st);
   if (rc) return rc;
-  return launch_dependent(few::extend_few_kernel<KM, VM, D>, few, grid, few::kFewThreads, few::FewLayout<KM, VM, D>::kBytes, st);
+  return launch_dependent<few::extend_few_kernel<KM, VM, D>>(few, grid, few::kFewThreads, few::FewLayout<KM, VM, D>::kBytes, st);
 }
 
 #define KNLP_EXTEND_PAIR(KM, VM)                                                              \

@@ -127,7 +127,13 @@ def _int4_mode(asymmetric: bool, zeros) -> int:
     return _lib.KV_INT4_SYM
 
 
+# The stream's handle without a Stream object around it: 0.1 instead of 2.2 us of every call.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(dev) -> int:
+    if _raw_stream is not None:
+        return _raw_stream(dev.index)
     return torch.cuda.current_stream(dev).cuda_stream
 
 
