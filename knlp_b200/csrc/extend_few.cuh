@@ -247,18 +247,23 @@ __global__ void __launch_bounds__(kFewThreads, 1) extend_few_kernel(const __grid
       const int from = wg * lower * 8, mine = wg ? groups - lower : lower;
       const int held = min(rows - from, mine * 8);
 
-      for (int j = 0; j < n; ++j, ++count) {
-        constexpr int kMine = kFewRows / 2;
-        const int token = (it.e.tile0 + j) * kTile + tok128;
-        const uint32_t b = count % kScoreBuffers;
-        wait(&mi.s_full[b], count / kScoreBuffers);
+      // The scores of the next tile are on their way while this one's P is handed over.
+      constexpr int kMine = kFewRows / 2;
+      float s[kMine];
+      auto ask = [&](uint32_t tile) {
+        const uint32_t b = tile % kScoreBuffers;
+        wait(&mi.s_full[b], tile / kScoreBuffers);
         fence_after();
-        float s[kMine];
         tmem_ld16(tmem + lanes + b * kFewRows + from, reinterpret_cast<uint32_t*>(s));
+      };
+      if (n) ask(count);
+#pragma unroll 1
+      for (int j = 0; j < n; ++j, ++count) {
+        const int token = (it.e.tile0 + j) * kTile + tok128;
         tmem_wait_ld16(reinterpret_cast<uint32_t*>(s));
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&mi.s_free[b]);
+        if (lane == 0) mbar_arrive(&mi.s_free[count % kScoreBuffers]);
         uint32_t pk[kMine / 2];
         if (mine) {
           if ((it.e.tile0 + j + 1) * kTile > least) {
@@ -330,6 +335,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) extend_few_kernel(const __grid
             }
           }
         }
+        if (j + 1 < n) ask(count + 1);
         wait(&mi.p_free, count + 1);  // the product with the last tile's P is done
 #pragma unroll
         for (int g = 0; g < kMine / 8; ++g) {
