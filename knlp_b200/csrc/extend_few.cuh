@@ -4,11 +4,12 @@
 //   S^T = K Q^T  (128 tokens x 32 rows),   P^T = exp2(c S^T - m),   O^T += V^T P^T  (head_dim x 32),
 //   l += 1 P^T  (a product with ones: every lane of the accumulator holds the column sums)
 //
-// What bounds it: HBM, and close behind it the conversion of the packed rows (a tile of 128
-// tokens is 20 KB, 890 cycles at the SM's share of the measured bandwidth, and 32 K values).  With
-// rows on M, as the kernel for many rows has them, 3/4 of the products and of the softmax lanes
-// would serve nothing, on two of the eight softmax warps; here a tile's products take 3 x 320
-// tensor cycles at N = 32 and all eight softmax warps share its exponentials.
+// What bounds it: a tile of 128 tokens is 20 KB, 890 cycles at the SM's share of the measured
+// bandwidth, and 32 K values to convert; measured 2200 cycles a tile with 65 % of the issue slots
+// taken (3-8 new tokens x 16 sequences on 8-32 K cached tokens, 32/8 heads of 128, INT4: 175 us,
+// 2.1 TB/s).  With rows on M, as the kernel for many rows has them, 3/4 of the products and of the
+// softmax lanes serve nothing, on two of its eight softmax warps: the same case takes 280 us there.
+// Here a tile's products take 3 x 320 tensor cycles at N = 32 and eight warps share its exponentials.
 //
 // One CTA per SM, 28 warps of at most 72 registers:
 //   warps 0-3, 4-7  softmax, a thread per token of the tile; the second warpgroup has the upper

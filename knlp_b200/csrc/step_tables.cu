@@ -6,11 +6,11 @@
 //   table[s, blocks(ctx_s) + j] = free[head + sum_{r<s} fresh_r + j],   0 <= j < fresh_s
 //   token i of request s: position ctx_s + i, slot = table[s, pos / bs] * bs + pos % bs
 //
-// What bounds it: latency.  A step of 32 requests moves 5 KB; only admissions of ~1e5 tokens
-// and more reach the memory system (16 bytes written per token).  So it is ONE launch without
-// any communication between blocks: every block scans the lengths of all requests itself
-// (8 bytes each, from L2), in chunks of kChunk, and serves the tokens and fresh table entries
-// of its own share that fall into the chunk.  A token finds its request by bisection in shared
+// What bounds it: latency.  A step of 32 requests moves 5 KB (3.5 us on the device); 1024 prompts
+// with 1.0 Mi tokens write 17 MB (15 us, 2.6 us at the copy rate: the blocks' scans).  ONE launch
+// without any communication between blocks: every block scans the lengths of all requests itself
+// (8 bytes each, from L2), in chunks of kChunk, and serves the tokens and fresh table entries of
+// its own share that fall into the chunk.  A token finds its request by bisection in shared
 // memory; its slot comes from the free list directly when the block is fresh, so that no block
 // reads a table entry that another one writes.
 

@@ -4,9 +4,11 @@
 //   m = max x,  l = sum e^(x-m),  w = sum e^(x-m) (x-m)
 //   logprob(t) = (x_t - m) - ln l,   entropy = ln l - w / l,   rank = 1 + #{i : x_i > x_t}
 //
-// What bounds it: HBM, the logits are read once (2 or 4 bytes each, against one exp2 and about
-// seven more instructions).  A thread keeps (m, l, w) of its own share online, in base-2 units;
-// they are merged at the end: with d = m_old - m, l' = l 2^d and w' = (w + d l) 2^d.
+// What bounds it: the logits are read once (2 or 4 bytes each) against one exp2 and about seven
+// more instructions: fp32 rows run at 5.3 TB/s without alternatives, bf16 rows at 3.5 (2047 rows
+// of 50257 with 8 alternatives: 68 us, 3.0 TB/s), by instruction issue.  A thread keeps (m, l, w)
+// of its own share online, in base-2 units; they are merged at the end: with d = m_old - m, l' = l
+// 2^d and w' = (w + d l) 2^d.
 //
 // The k largest come from the same pass: the k-th largest of the kGroups group maxima (a group =
 // a few threads' shares) is a bound that at least k elements reach, and hardly more than k do.
@@ -15,9 +17,10 @@
 // ties or a lopsided row overflow the collection, slower exact paths follow (below).  NaN counts
 // as the largest value, as in torch.
 //
-// A row is served by a cluster of 1, 2, 4 or 8 blocks, each with a slice; the first block merges
-// through distributed shared memory.  More than one block pays while rows x slices leave SMs
-// without work (launch_token_score).
+// Blocks of 256 threads: the ranking at a row's end runs under other rows' reading (512 threads:
+// 83 us on the same case).  A row is served by a cluster of 1, 2, 4 or 8 blocks, each with a
+// slice; the first block merges through distributed shared memory.  More than one block pays while
+// rows x slices leave SMs without work (launch_token_score).
 
 #include <cooperative_groups.h>
 
