@@ -409,7 +409,8 @@ int knlp_b200_decode_noalloc(const void* query, int q_dtype, const int64_t q_str
  *   block_table      as knlp_b200_decode_splitk; max_blocks entries per row.  A length above
  *                    max_blocks * block_size is cut there
  *   max_query_len    host-known bounds of the new tokens per sequence and of seq_lens.  They
- *   max_seq_len      choose how the work is split, never what is computed
+ *   max_seq_len      choose how the work is cut and what is launched, never what is computed:
+ *                    bounds given too small cost time only
  *   softmax_scale    factor of the scores, > 0 (head_dim^-1/2 as a rule)
  *   workspace        floats, >= what knlp_b200_extend_workspace reports; scratch.  Calls that
  *                    may overlap on the GPU need one each

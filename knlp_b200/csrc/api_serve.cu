@@ -78,7 +78,8 @@ int knlp_b200_extend_attention(const void* query, int q_dtype, const int64_t q_s
   a.out_row_stride = out_row_stride;
   a.lse = lse;
   if (!(flags & KNLP_EXTEND_FORCE_GENERIC)) {
-    rc = launch_extend_mma(a, workspace, workspace_floats, sm_count(), static_cast<cudaStream_t>(stream));
+    rc = launch_extend_mma(a, max_query_len, max_seq_len, workspace, workspace_floats, sm_count(),
+                           static_cast<cudaStream_t>(stream));
     if (rc <= 0) return rc;  // launched, or failed for good
   }
   return launch_extend_generic(a, static_cast<cudaStream_t>(stream));

@@ -26,12 +26,12 @@ constexpr int kSharedSeqs = 1024, kSharedTiles = 2048;
 // (query in, result out, an empty pipeline at both ends), and of the merging launch.
 constexpr float kItemCost = 4.0f, kMergeCost = 5.0f;
 
-// Sizes of a kernel's lists.  few: the tiles of at most 32 rows, one per sequence at most.
+// Sizes of a kernel's lists.
 struct Bounds {
   int64_t tiles, entries, parts;  // parts: rows of partial results
   Bounds(bool few, int n_seqs, int n_tokens, int n_q_heads, int n_kv_heads, int n_sms) {
     const int64_t rows = static_cast<int64_t>(n_tokens) * (n_q_heads / n_kv_heads);
-    tiles = few ? n_seqs : rows / kMaxRows + n_seqs;
+    tiles = rows / (few ? few::kFewRows : kMaxRows) + n_seqs;
     entries = 2 * tiles + 16 * static_cast<int64_t>(n_sms) / n_kv_heads + 2;
     // every row in pieces, up to a few tiles per SM
     const int64_t all = static_cast<int64_t>(n_tokens) * n_q_heads * 64;
@@ -50,7 +50,25 @@ struct Tile {
   }
 };
 
-__device__ Tile tile_at(const ExtendArgs& a, bool few_rows, int rep, const int* base, int t) {
+// What a batch is cut into.
+struct Cut {
+  bool few_rows;  // the list of the kernel for few rows
+  bool only_few;  // all rows go there, 32 at a time; else in tiles of 256, and what is left over
+  // Tiles of a sequence with that many rows.
+  __device__ int tiles_of(int64_t rows) const {
+    if (only_few) return few_rows ? static_cast<int>((rows + few::kFewRows - 1) / few::kFewRows) : 0;
+    const int rest = static_cast<int>(rows % kMaxRows);
+    const bool few = rest > 0 && rest <= few::kFewRows;
+    return few_rows ? few : static_cast<int>(rows / kMaxRows) + (rest > 0 && !few);
+  }
+  // First row of a tile, the i-th of its sequence.
+  __device__ int row0(int64_t rows, int i) const {
+    return only_few ? i * few::kFewRows : few_rows ? static_cast<int>(rows / kMaxRows) * kMaxRows : i * kMaxRows;
+  }
+  __device__ int most() const { return few_rows ? few::kFewRows : kMaxRows; }
+};
+
+__device__ Tile tile_at(const ExtendArgs& a, const Cut& cut, int rep, const int* base, int t) {
   int lo = 0, hi = a.n_seqs - 1;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
@@ -60,20 +78,13 @@ __device__ Tile tile_at(const ExtendArgs& a, bool few_rows, int rep, const int* 
   const int n = extend_rows(a, lo, &first), len = extend_length(a, lo);
   Tile x;
   x.seq = lo;
-  x.row0 = few_rows ? n * rep / kMaxRows * kMaxRows : (t - base[lo]) * kMaxRows;
-  x.rows = min(kMaxRows, n * rep - x.row0);
+  x.row0 = cut.row0(static_cast<int64_t>(n) * rep, t - base[lo]);
+  x.rows = min(cut.most(), n * rep - x.row0);
   const int last = (x.row0 + x.rows - 1) / rep;
   const int seen = a.causal ? max(min(a.seq_lens[lo] - n + last + 1, len), 0) : len;
   x.kv = (seen + kTile - 1) / kTile;
   return x;
 }
-// Tiles of a sequence with that many rows.
-__device__ int tiles_of(bool few_rows, int64_t rows) {
-  const int rest = static_cast<int>(rows % kMaxRows);
-  const bool few = rest > 0 && rest <= few::kFewRows;
-  return few_rows ? few : static_cast<int>(rows / kMaxRows) + (rest > 0 && !few);
-}
-
 // Exclusive prefix sums of N values over the block, and their totals.
 template <int N>
 __device__ void scan(int (&v)[N], int (&total)[N], int (*sh)[kPlanThreads / 32]) {
@@ -115,10 +126,10 @@ struct Lists {
 };
 
 __global__ void __launch_bounds__(kPlanThreads)
-extend_plan_kernel(const __grid_constant__ ExtendArgs a, int rep, int n_ctas, const __grid_constant__ Lists many,
-                   const __grid_constant__ Lists few) {
-  const bool few_rows = blockIdx.x;  // a block per kernel
-  const Lists& to = few_rows ? few : many;
+extend_plan_kernel(const __grid_constant__ ExtendArgs a, int rep, int n_ctas, bool only_few, bool whole,
+                   const __grid_constant__ Lists many, const __grid_constant__ Lists few) {
+  const Cut how{blockIdx.x == 1, only_few};  // a block per kernel
+  const Lists& to = how.few_rows ? few : many;
   // small batches are planned out of shared memory: every step of it is a latency
   __shared__ int sh_base[kSharedSeqs + 1];
   __shared__ int2 sh_tiles[kSharedTiles];  // (kv, rows)
@@ -134,7 +145,7 @@ extend_plan_kernel(const __grid_constant__ ExtendArgs a, int rep, int n_ctas, co
     const int s = s0 + tid;
     int first, v[1] = {0}, total[1];
     if (s < a.n_seqs) {
-      v[0] = tiles_of(few_rows, static_cast<int64_t>(extend_rows(a, s, &first)) * rep);
+      v[0] = how.tiles_of(static_cast<int64_t>(extend_rows(a, s, &first)) * rep);
     }
     scan(v, total, sh);
     if (s < a.n_seqs) base[s] = n_tiles + v[0];
@@ -146,13 +157,13 @@ extend_plan_kernel(const __grid_constant__ ExtendArgs a, int rep, int n_ctas, co
 
   float cost = 0.0f;
   for (int t = tid; t < n_tiles; t += kPlanThreads) {
-    const Tile x = tile_at(a, few_rows, rep, base, t);
+    const Tile x = tile_at(a, how, rep, base, t);
     cost += x.cost();
     if (t < kSharedTiles) sh_tiles[t] = make_int2(x.kv, x.rows);
   }
   // a tile as far as its cost goes
   auto size_of = [&](int t) {
-    if (t >= kSharedTiles) return tile_at(a, few_rows, rep, base, t);
+    if (t >= kSharedTiles) return tile_at(a, how, rep, base, t);
     Tile x{};
     x.kv = sh_tiles[t].x, x.rows = sh_tiles[t].y;
     return x;
@@ -167,7 +178,7 @@ extend_plan_kernel(const __grid_constant__ ExtendArgs a, int rep, int n_ctas, co
 
   // A candidate per warp: pieces of 1 / f of a CTA's equal share, or none (warp 0).
   const float share = cost * heads / n_ctas;
-  const float piece = warp == 0 ? 1e30f : fmaxf(share / (warp < 8 ? 0.5f * warp + 0.5f : warp - 3), 2.0f);
+  const float piece = warp == 0 || whole ? 1e30f : fmaxf(share / (warp < 8 ? 0.5f * warp + 0.5f : warp - 3), 2.0f);
   float worst = 0.0f;
   int items = 0;
   int64_t parts = 0;
@@ -227,7 +238,7 @@ extend_plan_kernel(const __grid_constant__ ExtendArgs a, int rep, int n_ctas, co
     Tile x{};
     int n = 0;
     if (t < n_tiles) {
-      x = tile_at(a, few_rows, rep, base, t);
+      x = tile_at(a, how, rep, base, t);
       n = x.pieces(c);
     }
     const int cut = n > 1 ? x.rows * heads : 0;
@@ -368,8 +379,8 @@ int64_t extend_workspace_floats(int n_seqs, int n_tokens, int n_q_heads, int n_k
   return extend::Sizes(n_seqs, n_tokens, n_q_heads, n_kv_heads, head_dim, n_sms).floats;
 }
 
-int launch_extend_mma(const ExtendArgs& a, float* ws, int64_t ws_floats, int n_sms,
-                      cudaStream_t st) {
+int launch_extend_mma(const ExtendArgs& a, int max_query_len, int max_seq_len, float* ws,
+                      int64_t ws_floats, int n_sms, cudaStream_t st) {
   using namespace extend;
   if (a.head_dim != 64 && a.head_dim != 128) return 1;
   if (!pair_built(a.k.mode, a.v.mode)) return 1;
@@ -406,12 +417,17 @@ int launch_extend_mma(const ExtendArgs& a, float* ws, int64_t ws_floats, int n_s
     for (int b = 0; b < 31; ++b)
       if (a.block_size == 1 << b) p[i].block_shift = b;
   }
-  extend_plan_kernel<<<2, kPlanThreads, 0, st>>>(a, p[0].rep, n_sms, lists[0], lists[1]);
+  // The host's bounds save launches; the plan keeps to what is launched, so bounds that are too
+  // small cost time, never rows or tokens.  Up to 32 rows per sequence: the kernel for many rows is
+  // left out and longer sequences are cut into 32s.  Up to three tiles of cached tokens: pieces
+  // are not made and the merge is left out.
+  const bool only_few = static_cast<int64_t>(max_query_len < a.n_tokens ? max_query_len : a.n_tokens) * p[0].rep <= few::kFewRows;
+  const bool whole = max_seq_len <= 3 * kTile;
+  extend_plan_kernel<<<2, kPlanThreads, 0, st>>>(a, p[0].rep, n_sms, only_few, whole, lists[0], lists[1]);
   if (cudaGetLastError() != cudaSuccess) return KNLP_ERR_LAUNCH;
-  // with at most 32 rows in all no sequence has more
-  const bool only_few = static_cast<int64_t>(a.n_tokens) * p[0].rep <= few::kFewRows;
   const int rc = launch_modes(p[0], p[1], only_few, n_sms, st);
   if (rc != KNLP_OK) return rc > 0 ? KNLP_ERR_MODE : rc;
+  if (whole) return KNLP_OK;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(2 * n_sms);
   cfg.blockDim = dim3(kMergeThreads);

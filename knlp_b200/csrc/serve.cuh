@@ -47,8 +47,8 @@ __device__ __forceinline__ int extend_rows(const ExtendArgs& a, int seq, int* fi
 
 // Tensor-core kernel (extend_plan.cu, extend_mma.cuh).  Returns KNLP_OK, 1 if the layout is not
 // one it addresses (nothing launched), < 0 on error.
-int launch_extend_mma(const ExtendArgs& a, float* ws, int64_t ws_floats, int n_sms,
-                      cudaStream_t st);
+int launch_extend_mma(const ExtendArgs& a, int max_query_len, int max_seq_len, float* ws,
+                      int64_t ws_floats, int n_sms, cudaStream_t st);
 int64_t extend_workspace_floats(int n_seqs, int n_tokens, int n_q_heads, int n_kv_heads,
                                 int head_dim, int n_sms);
 // Device-side status word shared by the kernels with bounded waits (decode_mma.cu).

@@ -249,6 +249,17 @@ def test_row_counts_around_the_kernels_border(d, hq, hkv, cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hints", [dict(max_query_len=1), dict(max_seq_len=1), dict(max_query_len=1, max_seq_len=1),
+                                   dict(max_query_len=0, max_seq_len=0), dict(max_query_len=9, max_seq_len=10 ** 6),
+                                   dict(max_query_len=10 ** 6, max_seq_len=300)])
+def test_the_hosts_bounds_do_not_change_the_result(hints, cuda_device):
+    """Bounds that are right, too small or too large."""
+    Batch(cuda_device, [3000, 0, 700, 5, 130], [9, 400, 1, 0, 33], 8, 2, 128, "int4_asym", seed=34).check(
+        out_dtype=torch.float32, **hints)
+    Batch(cuda_device, [100, 300, 20], [2, 1, 4], 8, 2, 64, "k8v8", seed=35).check(**hints)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("generic", GENERIC)
 def test_full_and_scale(generic, cuda_device):
     """Every query token over all cached tokens; other scales than head_dim^-1/2."""
