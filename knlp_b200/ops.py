@@ -39,6 +39,7 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 import os
+import threading
 from typing import Optional, Tuple
 
 import torch
@@ -697,6 +698,9 @@ def kfp16_vint8_decode(
 
 _extend_ws = {}  # (device index, stream) -> float workspace
 _extend_sizes = {}  # shape -> floats of knlp_b200_extend_workspace
+# Threads that share a stream share its workspace, and a call is several launches: they must not
+# come between one another's.
+_extend_lock = threading.Lock()
 
 
 def _extend_workspace(dev: torch.device, S: int, T: int, Hq: int, Hkv: int, d: int):
@@ -774,17 +778,18 @@ def extend_attention(
     if T and S:
         if block_table.shape[1] == 0:
             raise ValueError("block_table has no columns")
-        ws = _extend_workspace(dev, S, T, Hq, num_kv_heads, d)
         flags = (0 if causal else _lib.EXTEND_FULL) | (
             _lib.EXTEND_FORCE_GENERIC if force_generic else 0)
-        with _on(dev):
+        with _on(dev), _extend_lock:
+            ws = _extend_workspace(dev, S, T, Hq, num_kv_heads, d)
             rc = _lib.load().knlp_b200_extend_attention(
                 query.data_ptr(), _dt(query), _stride2(query), C.byref(k_plane),
                 C.byref(v_plane), block_table.data_ptr(), block_table.stride(0),
                 block_table.shape[1], seq_lens.data_ptr(), query_start_loc.data_ptr(),
                 num_blocks, S, T, Hq, num_kv_heads, d, block_size,
                 T if max_query_len is None else max_query_len,
-                block_table.shape[1] * block_size if max_seq_len is None else max_seq_len,
+                min(block_table.shape[1] * block_size if max_seq_len is None else max_seq_len,
+                    2 ** 31 - 1),
                 d ** -0.5 if softmax_scale is None else softmax_scale,
                 ws.data_ptr(), ws.numel(), out.data_ptr(), _dt(out), d,
                 lse.data_ptr() if lse is not None else None, flags, _stream(dev))

@@ -53,6 +53,8 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, top_k: int = 0
     if not ids.is_contiguous():
         ids = ids.contiguous()
     n = ids.numel()
+    if max(n, vocab) >= 2 ** 31:
+        raise ValueError("too many rows or too large a vocabulary")
     shape = tuple(token_ids.shape)
     logprob, entropy = torch.empty((2,) + shape, dtype=torch.float32, device=dev)
     rank = torch.empty(shape, dtype=torch.int32, device=dev)

@@ -435,6 +435,25 @@ def test_streams_and_graphs(cuda_device):
 
 
 @pytest.mark.gpu
+def test_threads_that_share_a_stream(cuda_device):
+    """Calls of several host threads on one stream share its workspace; each call's launches stay
+    together."""
+    from concurrent.futures import ThreadPoolExecutor
+    batches = [Batch(cuda_device, [3000 + 500 * i, 40], [5 + i, 90], 8, 2, 128, "int4_asym", seed=25 + i)
+               for i in range(4)]
+    want = [b.run() for b in batches]
+    torch.cuda.synchronize()
+
+    def calls(b):
+        return [b.run() for _ in range(40)]
+    with ThreadPoolExecutor(len(batches)) as pool:
+        got = list(pool.map(calls, batches))
+    torch.cuda.synchronize()
+    for outs, w in zip(got, want):
+        assert all(torch.equal(o, w) for o in outs)
+
+
+@pytest.mark.gpu
 def test_step_of_a_batch_through_the_cache(cuda_device):
     """The pieces as a server uses them: tables from lengths, write, attend, over several steps
     of prefill chunks, drafted tokens and single tokens; compared with the oracle's attention
