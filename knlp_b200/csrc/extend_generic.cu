@@ -85,8 +85,9 @@ extend_generic_kernel(const ExtendArgs a, int n_rep, int q_groups) {
 #pragma unroll
     for (int h = 0; h < QH; ++h) {
       const float m_new = fmaxf(m[h], s[h]);
-      const float alpha = __expf(m[h] - m_new);  // exp(-inf) = 0 on the first token
-      const float pr = __expf(s[h] - m_new);
+      // a score of -inf weighs nothing, also while there is no other one (-inf - -inf)
+      const float alpha = m[h] == m_new ? 1.0f : __expf(m[h] - m_new);
+      const float pr = s[h] == -INFINITY ? 0.0f : __expf(s[h] - m_new);
       l[h] = l[h] * alpha + pr;
 #pragma unroll
       for (int i = 0; i < EPL; ++i) acc[h][i] = acc[h][i] * alpha + pr * kv[i];

@@ -108,8 +108,9 @@ class Batch:
             return ops.kint8_vint4_extend(self.query, self.k, self.v, self.ks, self.vs, *rest, **vz, **kw)
         return ops.kfp16_vint4_extend(self.query, self.k, self.v, self.vs, *rest, **vz, **kw)
 
-    def reference(self, causal=True, scale=None):
-        """(o, lse, bound of o, bound of lse) in 64 bits, rows [T, hq].
+    def reference(self, causal=True, scale=None, without=()):
+        """(o, lse, bound of o, bound of lse) in 64 bits, rows [T, hq], `without` tokens at some
+        positions.
 
         The bound: K and V are rounded to fp16 after dequantization, a bf16 Q below 2^-14 and P
         to fp16 (each within 2^-11 of its value or 2^-25), products are summed in fp32,
@@ -142,6 +143,7 @@ class Batch:
                 last = lens[s] - (b - a) + torch.arange(b - a, device=dev)
                 off = torch.arange(n, device=dev)[None] > last[:, None]
                 w, e = w.masked_fill(off, -math.inf), e.masked_fill(off, 0)
+            w[..., list(without)], e[..., list(without)] = -math.inf, 0
             ls = torch.logsumexp(w, -1)
             p = torch.exp(w - torch.where(ls.isinf(), 0, ls)[..., None])
             worst = e.amax(-1)
@@ -358,6 +360,23 @@ def test_values_that_are_not_finite_reach_only_the_rows_that_see_them(mode, many
     fine = (r - o).abs() <= bo + 2.0 ** -23 * o.abs()
     assert torch.isnan(r[see]).all()
     assert fine[~see].all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("generic", GENERIC)
+@pytest.mark.parametrize("ctx,new", [(200, 3), (200, 150)])
+def test_scores_of_minus_infinity_weigh_nothing(ctx, new, generic, cuda_device):
+    """Keys that are -inf in one element, under queries that are positive there: as if their
+    tokens were masked, wherever they lie (the first tokens, a run within a tile)."""
+    b = Batch(cuda_device, [ctx], [new], 4, 2, 64, "kfpv8", "f16", seed=18)
+    b.query[..., 7] = b.query[..., 7].abs() + 0.125
+    hit = [0, 1, 2, 3, 5, 64] + list(range(130, 150))
+    o, lse, bo, bl = b.reference(without=hit)
+    for t in hit:
+        b.k[int(b.table[0, t // 16]), t % 16, :, 7] = -math.inf
+    r, l = b.run(force_generic=generic, return_lse=True, out_dtype=torch.float32)
+    assert ((r.double() - o).abs() <= bo + 2.0 ** -24 * (o.abs() + bo)).all()
+    assert ((l.double() - lse).abs() <= bl).all()
 
 
 @pytest.mark.gpu
