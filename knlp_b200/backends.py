@@ -567,8 +567,7 @@ class PackedQuantBackend(QuantBackend):
                     at += rows.shape[1]
         if not parts:
             return scoring.token_logprobs(logits[:, :0], continuation_ids, top_k), stats
-        cat = [None if f[0] is None else torch.cat(f, dim=1) for f in zip(*parts)]
-        return scoring.TokenScores(*cat), stats
+        return scoring.TokenScores(*(torch.cat(f, dim=1) for f in zip(*parts))), stats
 
     def description(self):
         return "packed far cache: " + super().description()

@@ -9,7 +9,7 @@ vocabulary in fp32 (compute_ppl of its harnesses).  CUDA tensors only.
 
 from __future__ import annotations
 
-from typing import NamedTuple, Optional
+from typing import NamedTuple
 
 import torch
 
@@ -20,8 +20,8 @@ class TokenScores(NamedTuple):
     logprob: torch.Tensor  # fp32 [...]
     entropy: torch.Tensor  # fp32 [...], nats
     rank: torch.Tensor  # int32 [...], 1 = no logit is larger
-    top_ids: Optional[torch.Tensor]  # int64 [..., k], descending, lower index first among equals
-    top_logprobs: Optional[torch.Tensor]  # fp32 [..., k]
+    top_ids: torch.Tensor  # int64 [..., k], descending, lower index first among equals
+    top_logprobs: torch.Tensor  # fp32 [..., k]
 
 
 def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, top_k: int = 0) -> TokenScores:
@@ -58,10 +58,8 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, top_k: int = 0
     shape = tuple(token_ids.shape)
     logprob, entropy = torch.empty((2,) + shape, dtype=torch.float32, device=dev)
     rank = torch.empty(shape, dtype=torch.int32, device=dev)
-    top_ids = top_lp = None
-    if top_k:
-        top_ids = torch.empty(shape + (top_k,), dtype=torch.int64, device=dev)
-        top_lp = torch.empty(shape + (top_k,), dtype=torch.float32, device=dev)
+    top_ids = torch.empty(shape + (top_k,), dtype=torch.int64, device=dev)
+    top_lp = torch.empty(shape + (top_k,), dtype=torch.float32, device=dev)
     if n:
         with ops._on(dev):
             rc = _lib.load().knlp_b200_token_score(

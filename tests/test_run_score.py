@@ -46,6 +46,8 @@ def test_scores_are_those_of_run_decode(name, batch, cuda_device):
         if name == "quant_packed":
             assert stats[0].n_compressed == 84 and stats[-1].n_full == 36 + 9
             assert model.config._attn_implementation != "knlp_b200_packed"
+    s, _ = b.run_score(model, prefix, cont, str(cuda_device), 512)
+    assert s.rank.shape == (batch, 9) and s.top_ids.shape == (batch, 9, 0)
 
 
 def test_short_inputs_and_refusals(cuda_device):

@@ -49,11 +49,10 @@ def check(dev, x, ids, k, dtype):
     near(r.logprob, lp, tol)
     near(r.entropy, ent, tol * (1 + ent.max(initial=0)))
     assert np.array_equal(r.rank.cpu().numpy(), rank)
+    assert r.top_ids.shape == r.top_logprobs.shape == (len(xv), k)
     if k:
         assert np.array_equal(r.top_ids.cpu().numpy(), order)
         near(r.top_logprobs, top, tol)
-    else:
-        assert r.top_ids is None and r.top_logprobs is None
 
 
 @pytest.mark.gpu
