@@ -129,9 +129,9 @@ def build_step(context_lens: torch.Tensor, query_lens: torch.Tensor, block_table
     if block_size <= 0 or num_tokens < 0:
         raise ValueError("block_size must be positive and num_tokens not negative")
     small = torch.empty(2 * S + 2, dtype=torch.int32, device=dev)
-    wide = torch.empty((2, num_tokens), dtype=torch.int64, device=dev)
-    starts, lens, taken = small[:S + 1], small[S + 1:2 * S + 1], small[2 * S + 1:]
-    slots, positions = wide.unbind(0)
+    starts, lens, taken = small.split_with_sizes((S + 1, S, 1))
+    slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
+    positions = torch.empty_like(slots)
     with ops._on(dev):
         rc = _lib.load().knlp_b200_build_step(
             context_lens.data_ptr(), query_lens.data_ptr(), block_table.data_ptr(),

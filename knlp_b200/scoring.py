@@ -56,7 +56,8 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, top_k: int = 0
     if max(n, vocab) >= 2 ** 31:
         raise ValueError("too many rows or too large a vocabulary")
     shape = tuple(token_ids.shape)
-    logprob, entropy = torch.empty((2,) + shape, dtype=torch.float32, device=dev)
+    logprob = torch.empty(shape, dtype=torch.float32, device=dev)
+    entropy = torch.empty_like(logprob)
     rank = torch.empty(shape, dtype=torch.int32, device=dev)
     top_ids = torch.empty(shape + (top_k,), dtype=torch.int64, device=dev)
     top_lp = torch.empty(shape + (top_k,), dtype=torch.float32, device=dev)
