@@ -34,6 +34,7 @@ namespace few {
 constexpr int kFewRows = 32;
 constexpr int kFewThreads = 28 * 32;
 constexpr int kScoreBuffers = 4;
+constexpr float kLowest = -8192.0f;  // of scores in powers of two; sums with it keep 2^-11
 
 // TMEM columns: four buffers of S^T, O^T, l, and a tile of ones (fp16 pairs) as an operand.
 constexpr int kTmemO = kScoreBuffers * kFewRows, kTmemL = kTmemO + kFewRows, kTmemOnes = kTmemL + kFewRows;
@@ -297,7 +298,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) extend_few_kernel(const __grid
               const int x = from + tok128;
               float v = -INFINITY;
               if (tok128 < held) v = fmaxf(fmaxf(mi.most[0][x], mi.most[1][x]), fmaxf(mi.most[2][x], mi.most[3][x]));
-              const float by = j == 0 ? (v == -INFINITY ? 0.0f : v) : fmaxf(v, 0.0f);
+              // a row whose scores are all -inf so far: a real one will lie above its reference
+              const float first = v > -INFINITY ? v : tok128 < held ? kLowest : 0.0f;
+              const float by = j == 0 ? first : fmaxf(v, 0.0f);
               mi.delta[x] = by;
               mi.factor[x] = exp2f(-by);
               mi.off[x] -= by;

@@ -364,13 +364,14 @@ def test_values_that_are_not_finite_reach_only_the_rows_that_see_them(mode, many
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("generic", GENERIC)
-@pytest.mark.parametrize("ctx,new", [(200, 3), (200, 150)])
-def test_scores_of_minus_infinity_weigh_nothing(ctx, new, generic, cuda_device):
+@pytest.mark.parametrize("ctx,new,first", [(200, 3, 4), (200, 150, 4), (5000, 3, 200), (700, 3, 129),
+                                           (300, 150, 129)])
+def test_scores_of_minus_infinity_weigh_nothing(ctx, new, first, generic, cuda_device):
     """Keys that are -inf in one element, under queries that are positive there: as if their
-    tokens were masked, wherever they lie (the first tokens, a run within a tile)."""
+    tokens were masked, wherever they lie (the first tokens, whole tiles, a run within one)."""
     b = Batch(cuda_device, [ctx], [new], 4, 2, 64, "kfpv8", "f16", seed=18)
     b.query[..., 7] = b.query[..., 7].abs() + 0.125
-    hit = [0, 1, 2, 3, 5, 64] + list(range(130, 150))
+    hit = list(range(first)) + [first + 1, 64] + list(range(130, 150))
     o, lse, bo, bl = b.reference(without=hit)
     for t in hit:
         b.k[int(b.table[0, t // 16]), t % 16, :, 7] = -math.inf
