@@ -8,7 +8,7 @@
 // What bounds it: a 128 x 128 tile costs 2 x 512 tensor cycles at head_dim 128 and 1024 cycles of
 // the SM's 16 ex2 per cycle; measured, the chain of a softmax step (TMEM load, maximum,
 // exponentials, TMEM store, hand-over) beside them: 4096 new tokens at 28 000 cached ones, 32/8
-// heads of 128, INT4: 2.19 ms, 920 TFLOP/s, 49 % tensor pipe, 49 % special function unit, 59 % issue slots.  Work
+// heads of 128, INT4: 2.19 ms, 910 TFLOP/s, 49 % tensor pipe, 49 % special function unit, 59 % issue slots.  Work
 // items and their split over CTAs: extend_plan.cu.
 //
 // One CTA per SM (it owns all 512 TMEM columns), 20 warps whose registers are dealt out by
